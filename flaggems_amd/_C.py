@@ -18,6 +18,8 @@ LIB_PATH = os.environ.get("FG_LIB_PATH") or os.path.join(_HERE, "libfg_mi355.so"
 FG_F16, FG_BF16, FG_F32 = 0, 1, 2
 SCHED_AUTO, SCHED_DATA_PARALLEL, SCHED_STREAM_K = 0, 1, 2
 
+CACHE_SAME, CACHE_E4M3, CACHE_E5M2 = 0, 1, 2
+
 _DTYPE_ID = {torch.float16: FG_F16, torch.bfloat16: FG_BF16, torch.float32: FG_F32}
 
 c_i64 = ctypes.c_int64
@@ -71,6 +73,24 @@ class FgFlashParams(ctypes.Structure):
     ]
 
 
+class FgCacheAttnParams(ctypes.Structure):
+    """Mirror of struct FgCacheAttnParams in include/fg_mi355.h."""
+
+    _fields_ = [
+        ("base", FgFlashParams),
+        ("cache_format", ctypes.c_int32),
+        ("num_sink_tokens", ctypes.c_int32),
+        ("num_pages", c_i64),
+        ("table_width", ctypes.c_int32),
+        ("k_scale", c_vp),
+        ("v_scale", c_vp),
+        ("k_scale_batch_stride", c_i64),
+        ("k_scale_head_stride", c_i64),
+        ("v_scale_batch_stride", c_i64),
+        ("v_scale_head_stride", c_i64),
+    ]
+
+
 _SIGNATURES = {
     "fg_last_error": (ctypes.c_char_p, []),
     "fg_abi_version": (c_int, []),
@@ -93,6 +113,16 @@ _SIGNATURES = {
     "fg_reshape_and_cache": (
         c_int,
         [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_int, c_int, c_int, c_int, c_i64, c_i64, c_i64, c_int, c_vp],
+    ),
+    "fg_reshape_and_cache_flash_8bit": (
+        c_int,
+        [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_int, c_int, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64,
+         c_vp, c_i64, c_int, c_int, c_vp],
+    ),
+    "fg_gather_cache_flash": (
+        c_int,
+        [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_i64, c_int, c_int, c_int, c_i64, c_i64, c_i64,
+         c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_int, c_vp],
     ),
     "fg_silu_and_mul": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]),
     "fg_silu_and_mul_backward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
@@ -134,6 +164,8 @@ _SIGNATURES = {
     ),
     "fg_flash_attn_varlen_fwd": (c_int, [ctypes.POINTER(FgFlashParams), c_vp]),
     "fg_flash_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FgFlashParams), c_int]),
+    "fg_cache_attn_fwd": (c_int, [ctypes.POINTER(FgCacheAttnParams), c_vp]),
+    "fg_cache_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FgCacheAttnParams), c_int]),
 }
 
 _lib = None
@@ -189,6 +221,59 @@ def dtype_id(dtype):
         return _DTYPE_ID[dtype]
     except KeyError:
         raise TypeError("dtype %s is not supported by the gfx950 kernels (fp16, bf16, fp32 only)" % dtype)
+
+
+# 8-bit caches: the format a torch type stands for, and the formats that a kv_cache_dtype names (a cache of plain bytes
+# has no type of its own)
+_CACHE_FORMAT = {torch.float8_e4m3fn: CACHE_E4M3, torch.float8_e5m2: CACHE_E5M2}
+CACHE_8BIT = (torch.float8_e4m3fn, torch.float8_e5m2, torch.uint8)
+_CACHE_NAMES = {"fp8": CACHE_E4M3, "fp8_e4m3": CACHE_E4M3, "fp8_e5m2": CACHE_E5M2}
+
+
+def cache_format(cache_dtype, kv_cache_dtype="auto"):
+    """Format id of an 8-bit cache, or None for a cache of any other type."""
+    if cache_dtype == torch.uint8:
+        if kv_cache_dtype not in _CACHE_NAMES:
+            raise ValueError("a cache of bytes needs kv_cache_dtype fp8, fp8_e4m3 or fp8_e5m2, got %r" % (kv_cache_dtype,))
+        return _CACHE_NAMES[kv_cache_dtype]
+    fmt = _CACHE_FORMAT.get(cache_dtype)
+    if fmt is not None and _CACHE_NAMES.get(kv_cache_dtype, fmt) != fmt:
+        raise ValueError("kv_cache_dtype %r does not fit a cache of %s" % (kv_cache_dtype, cache_dtype))
+    return fmt
+
+
+def head_scale(scale, heads, device, name):
+    """(pointer, head stride) of an fp32 scale tensor: one number, or one for each head.  None: no scale (1)."""
+    if scale is None:
+        return None, 0
+    _check_scale(scale, device, name)
+    if scale.numel() == 1:
+        return scale.data_ptr(), 0
+    if scale.shape != (heads,) or scale.stride(0) != 1:
+        raise ValueError("%s must hold one number or a contiguous one for each of the %d heads, got shape %s" % (
+            name, heads, tuple(scale.shape)))
+    return scale.data_ptr(), 1
+
+
+def sequence_scale(scale, batch, heads, device, name):
+    """(pointer, batch stride, head stride) of an fp32 scale tensor that expands to (batch, heads).  None: no scale (1)."""
+    if scale is None:
+        return None, 0, 0
+    _check_scale(scale, device, name)
+    if scale.numel() == 1:
+        return scale.data_ptr(), 0, 0
+    try:
+        full = scale.expand(batch, heads)
+    except RuntimeError:
+        raise ValueError("%s must expand to (batch, kv heads) = (%d, %d), got shape %s" % (name, batch, heads, tuple(scale.shape)))
+    return full.data_ptr(), full.stride(0), full.stride(1)
+
+
+def _check_scale(scale, device, name):
+    if not isinstance(scale, torch.Tensor):
+        raise TypeError("%s must be a tensor, got %s" % (name, type(scale).__name__))
+    if scale.dtype != torch.float32 or scale.device != device:
+        raise ValueError("%s must be float32 on %s, got %s on %s" % (name, device, scale.dtype, scale.device))
 
 
 def supported_dtype(dtype):

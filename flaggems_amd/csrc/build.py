@@ -30,12 +30,14 @@ SOURCES = [
     "transpose.hip",
     "rope.hip",
     "kvcache.hip",
+    "kvcache_8bit.hip",
     "silu_mul.hip",
     "gemm.hip",
     "gemm_skinny.hip",
     "gemm_streamk.hip",
     "gemm_dma.hip",
     "attn_varlen.hip",
+    "attn_cache.hip",
     "probe.hip",
 ]
 

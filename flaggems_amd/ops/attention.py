@@ -141,6 +141,72 @@ def mha_varlan_fwd(
     return out, q, k, v, lse, philox_args, unused, probs
 
 
+def cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, page_table, alibi_slopes, max_seqlen_q, max_seqlen_k,
+                   softmax_scale, is_causal, window_size_left, window_size_right, softcap, num_sink_tokens, k_descale,
+                   v_descale):
+    """Attention over an 8-bit paged cache, or under a window with sink tokens: validation + launch.  Returns (out, lse)."""
+    assert q.is_cuda and k.is_cuda and v.is_cuda
+    assert q.dtype in (torch.float16, torch.bfloat16), "FlashAttention only support fp16 and bf16 data type"
+    assert k.dtype == v.dtype
+    fmt = _C.cache_format(k.dtype)
+    assert fmt is not None or k.dtype == q.dtype, "the cache must hold q's type or 8-bit floats"
+    total_q, num_heads, head_size = q.shape
+    num_pages, block_size, num_heads_k, _ = k.shape
+    batch = cu_seqlens_q.numel() - 1
+    assert k.shape == v.shape == (num_pages, block_size, num_heads_k, head_size)
+    for t in (q, k, v):
+        assert t.stride(-1) == 1, "Input tensor must have contiguous last dimension"
+    assert page_table is not None and page_table.dtype == torch.int32 and page_table.dim() == 2
+    assert page_table.stride(-1) == 1 or page_table.size(1) <= 1
+    assert page_table.size(0) >= batch and page_table.size(1) > 0
+    assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.dim() == 1
+    assert seqused_k is not None, "the paged kernel takes key lengths from seqused_k"
+    assert seqused_k.dtype == torch.int32 and seqused_k.is_contiguous() and seqused_k.shape == (batch,)
+    assert num_heads % num_heads_k == 0, "Number of heads in key/value must divide number of heads in query"
+    assert num_sink_tokens >= 0, "num_sink_tokens must not be negative"
+    for t in (k, v, page_table, cu_seqlens_q, seqused_k, out):
+        assert t is None or t.device == q.device, "all tensors must be on one device"
+    if alibi_slopes is not None:
+        raise NotImplementedError("alibi_slopes are not supported with an 8-bit cache or sink tokens")
+    if out is not None:
+        assert out.stride(-1) == 1 and out.dtype == q.dtype and out.shape == (total_q, num_heads, head_size)
+    with _C.device_guard(q.device):
+        if out is None:
+            out = torch.empty((total_q, num_heads, head_size), dtype=q.dtype, device=q.device)
+        lse = torch.empty((num_heads, total_q), dtype=torch.float, device=q.device)
+        if total_q > 0 and batch > 0:
+            c = _C.FgCacheAttnParams()
+            p = c.base
+            p.q, p.k_cache, p.v_cache, p.out, p.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
+            p.cu_seqlens_q, p.seqused_k, p.block_table = cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), page_table.data_ptr()
+            p.q_row_stride, p.q_head_stride, _ = q.stride()
+            p.o_row_stride, p.o_head_stride, _ = out.stride()
+            p.k_page_stride, p.k_row_stride, p.k_head_stride, _ = k.stride()
+            p.v_page_stride, p.v_row_stride, p.v_head_stride, _ = v.stride()
+            p.block_table_stride = page_table.stride(0)
+            p.total_q = total_q
+            p.batch, p.Hq, p.Hk, p.D, p.page_size = batch, num_heads, num_heads_k, head_size, block_size
+            p.max_seqlen_q, p.max_seqlen_k = int(max_seqlen_q), int(max_seqlen_k)
+            p.is_causal = 1 if is_causal else 0
+            p.window_left, p.window_right = int(window_size_left), int(window_size_right)
+            p.softmax_scale, p.softcap = float(softmax_scale), float(softcap)
+            p.dtype = _C.dtype_id(q.dtype)
+            c.cache_format = _C.CACHE_SAME if fmt is None else fmt
+            c.num_sink_tokens, c.num_pages, c.table_width = int(num_sink_tokens), num_pages, page_table.size(1)
+            if fmt is not None:
+                c.k_scale, c.k_scale_batch_stride, c.k_scale_head_stride = _C.sequence_scale(
+                    k_descale, batch, num_heads_k, q.device, "k_descale")
+                c.v_scale, c.v_scale_batch_stride, c.v_scale_head_stride = _C.sequence_scale(
+                    v_descale, batch, num_heads_k, q.device, "v_descale")
+            ws_bytes = _C.lib().fg_cache_attn_workspace_bytes(ctypes.byref(c), q.device.index or 0)
+            if ws_bytes > 0:
+                ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+                p.workspace, p.workspace_bytes = ws.data_ptr(), ws_bytes
+            rc = _C.lib().fg_cache_attn_fwd(ctypes.byref(c), _C.current_stream(q.device))
+            _C.check(rc, "fg_cache_attn_fwd")
+    return out, lse
+
+
 def flash_attn_varlen_func(
     q,
     k,
@@ -169,6 +235,7 @@ def flash_attn_varlen_func(
     v_descale=None,
     num_splits: int = 0,
     fa_version: int = 2,
+    num_sink_tokens: int = 0,
 ):
     """Variable-length attention forward with FA2 semantics over a paged KV cache.
 
@@ -180,7 +247,15 @@ def flash_attn_varlen_func(
     (nheads,) or (batch, nheads) fp32 adds -slope * |i + seqlen_k - seqlen_q - j|.
     Returns out (total_q, nheads, headdim), and the fp32 log-sum-exp (nheads, total_q) as well
     when return_softmax_lse is set.  q_v, deterministic, return_attn_probs, scheduler_metadata
-    and the descale arguments are accepted and ignored, as in the reference.
+    and, for a cache of q's own type, the descale arguments are accepted and ignored, as in the reference.
+
+    An 8-bit cache (k and v of torch.float8_e4m3fn or torch.float8_e5m2, head dim a multiple of 16; a cache of bytes is
+    passed as a view of one of these types) stands for k * k_descale and v * v_descale: float32 tensors that expand to
+    (batch, nheads_k), None for 1.  q stays in 16 bits (q_descale must be None).
+    num_sink_tokens: the first keys of a sequence stay visible in front of a left window (key j is visible if it lies in the
+    window or j < num_sink_tokens, and the causal or right bound admits it); pages outside both are not read and may be gone.
+    Neither goes together with alibi_slopes.  A block table entry that is needed and names no page of the cache gives NaN;
+    so does an infinite or NaN value, for the queries that see its key and for others that share their block of rows.
     """
     logger.debug("GEMS FLASH_ATTN_VARLEN_FUNC")
     assert cu_seqlens_k is not None or seqused_k is not None, "cu_seqlens_k or seqused_k must be provided"
@@ -200,6 +275,16 @@ def flash_attn_varlen_func(
         raise RuntimeError("num_splits > 0 is not implemented in GEMS.")
     max_seqlen_q = max_seqlen_q.item() if hasattr(max_seqlen_q, "item") else max_seqlen_q
     max_seqlen_k = max_seqlen_k.item() if hasattr(max_seqlen_k, "item") else max_seqlen_k
+    left, right = real_window_size
+    if k.dtype in _C.CACHE_8BIT or (num_sink_tokens != 0 and left >= 0):
+        assert dropout_p == 0, "dropout is not implemented on this path (inference only)"
+        if k.dtype in _C.CACHE_8BIT and q_descale is not None:
+            raise NotImplementedError("q_descale: the query is not quantized on this path")
+        out, softmax_lse = cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, block_table, alibi_slopes, max_seqlen_q,
+                                          max_seqlen_k, softmax_scale, causal, left, right, softcap, num_sink_tokens,
+                                          k_descale, v_descale)
+        return (out, softmax_lse) if return_softmax_lse else out
+    assert num_sink_tokens >= 0, "num_sink_tokens must not be negative"
     out, q, k, v, softmax_lse, *_ = mha_varlan_fwd(
         q, k, v, out, cu_seqlens_q,
         # (the reference passes an uninitialised tensor shaped like cu_seqlens_q here; only its shape and dtype are

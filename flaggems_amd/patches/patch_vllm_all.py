@@ -94,6 +94,7 @@ def custom_gems_flash_attention_impl_forward(
 ) -> torch.Tensor:
     """v1 FlashAttentionImpl.forward: append this step's K/V to the paged cache, then attend over it.
     query [tokens, heads, d]; kv_cache [2, pages, page_size, kv_heads, d]; writes output[:num_actual_tokens]."""
+    from .. import _C
     from ..fused.reshape_and_cache_flash import reshape_and_cache_flash
     from ..ops.attention import flash_attn_varlen_func
 
@@ -102,10 +103,13 @@ def custom_gems_flash_attention_impl_forward(
         raise NotImplementedError("fused output quantization is not yet supported for FlashAttentionImpl")
     if attn_metadata is None:  # memory-profiling pass
         return output
-    if self.kv_cache_dtype.startswith("fp8"):
-        raise NotImplementedError("FP8 quantization is not yet supported for FlashAttentionImpl")
+    quantized = self.kv_cache_dtype.startswith("fp8")
+    if quantized and getattr(kv_cache, "dtype", None) not in _C.CACHE_8BIT:
+        raise NotImplementedError("kv_cache_dtype %s needs a cache of 8-bit elements" % self.kv_cache_dtype)
 
     n = attn_metadata.num_actual_tokens
+    if quantized and kv_cache.dtype == torch.uint8:
+        kv_cache = kv_cache.view(torch.float8_e5m2 if self.kv_cache_dtype == "fp8_e5m2" else torch.float8_e4m3fn)
     key_cache, value_cache = kv_cache.unbind(0)
     reshape_and_cache_flash(
         key, value, key_cache, value_cache, attn_metadata.slot_mapping, self.kv_cache_dtype,
@@ -129,7 +133,8 @@ def custom_gems_flash_attention_impl_forward(
         cu_seqlens_q=cu_q, max_seqlen_q=max_q, seqused_k=used_k, max_seqlen_k=max_k,
         softmax_scale=self.scale, causal=True, alibi_slopes=self.alibi_slopes, window_size=self.sliding_window,
         block_table=table, softcap=self.logits_soft_cap, scheduler_metadata=sched, fa_version=2,
-        q_descale=layer._q_scale.expand(descale_shape), k_descale=layer._k_scale.expand(descale_shape),
+        q_descale=None if quantized else layer._q_scale.expand(descale_shape),  # (the query stays in 16 bits)
+        k_descale=layer._k_scale.expand(descale_shape),
         v_descale=layer._v_scale.expand(descale_shape),
     )
     return output

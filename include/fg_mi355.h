@@ -133,6 +133,34 @@ int fg_reshape_and_cache_flash(const void* key, const void* value, void* key_cac
                                int64_t key_stride, int64_t value_stride, int64_t block_stride,
                                int elem_bytes, void* stream);
 
+/* What a paged cache holds: values of the operator's own type, or 8-bit floats (OCP e4m3 without infinities, e5m2). */
+enum { FG_CACHE_SAME = 0, FG_CACHE_E4M3 = 1, FG_CACHE_E5M2 = 2 };
+
+/* The scatter into an 8-bit cache: c = rn8(clamp(x / scale, -max, max)), NaN stays NaN.  key/value: rows of H*D dense
+ * elements of `dtype` at the given token strides; caches [num_blocks, block_size, H, D] of bytes with dense pages and the
+ * given block strides.  k_scale / v_scale: device fp32, NULL = 1, one number (stride 0) or one for each head (stride 1).
+ * Slots < 0 and slots past the last block are skipped; slots must differ.
+ * The reference's reshape_and_cache_flash takes kv_cache_dtype and the scales and ignores them
+ * (src/flag_gems/fused/reshape_and_cache_flash.py:61-112). */
+int fg_reshape_and_cache_flash_8bit(const void* key, const void* value, void* key_cache, void* value_cache,
+                                    const void* slot_mapping, int slot_is_i64, int64_t num_tokens, int H, int D,
+                                    int block_size, int64_t num_blocks, int64_t key_stride, int64_t value_stride,
+                                    int64_t key_block_stride, int64_t value_block_stride, const float* k_scale,
+                                    int64_t k_scale_stride, const float* v_scale, int64_t v_scale_stride, int dtype,
+                                    int cache_format, void* stream);
+
+/* Reads sequences back from a paged cache as packed rows: row r with cu_seqlens[b] <= r < cu_seqlens[b + 1] of key / value
+ * [num_rows, H, D] (`dtype`) is position r - cu_seqlens[b] + seq_starts[b] of sequence b (seq_starts NULL: 0), times the
+ * scale for an 8-bit cache, a plain copy for FG_CACHE_SAME.  Rows that belong to no sequence are left as they were; a
+ * position whose page is not in the table or not in the cache gives zeros.  Caches [num_pages, page_size, H, D] with dense
+ * pages, strides in elements.  No counterpart in the reference. */
+int fg_gather_cache_flash(const void* key_cache, const void* value_cache, void* key, void* value,
+                          const int32_t* block_table, int64_t block_table_stride, int table_width,
+                          const int32_t* cu_seqlens, const int32_t* seq_starts, int batch, int64_t num_rows, int H, int D,
+                          int page_size, int64_t num_pages, int64_t key_page_stride, int64_t value_page_stride,
+                          int64_t key_stride, int64_t value_stride, const float* k_scale, int64_t k_scale_stride,
+                          const float* v_scale, int64_t v_scale_stride, int dtype, int cache_format, void* stream);
+
 /* The same scatter into the older cache layout: key_cache [num_blocks, H, D/x, block_size, x] and
  * value_cache [num_blocks, H, D, block_size], both contiguous; key/value [num_tokens, H, D] with a dense
  * [H, D] block per token and the given token strides (elements).  Slots < 0 and slots past the last block
@@ -276,6 +304,30 @@ int fg_flash_attn_varlen_fwd(const FgFlashParams* p /*host*/, void* stream);
  * src/flag_gems/ops/flash_api.py:752-800).  The forward never needs it: without it (NULL or too
  * small) it runs unsplit.  Uninitialised memory is fine; one stream at a time. */
 size_t fg_flash_attn_workspace_bytes(const FgFlashParams* p /*host*/, int device);
+
+/* fg_flash_attn_varlen_fwd over a cache that holds 8-bit values, or under a sliding window with first tokens that stay
+ * visible, or both. */
+typedef struct FgCacheAttnParams {
+  FgFlashParams base;       /* as above; dtype is that of q and out; alibi_slopes must be NULL; workspace: see below.
+                               K and V strides are elements of the cache.  With an 8-bit cache D is a multiple of 16. */
+  int32_t cache_format;     /* FG_CACHE_SAME: the cache has q's type */
+  int32_t num_sink_tokens;  /* keys j < num_sink_tokens stay visible in front of a left window */
+  int64_t num_pages;        /* pages of the caches */
+  int32_t table_width;      /* entries of a block table row */
+  const float* k_scale;     /* device fp32, what the cached K / V were divided by; NULL = 1; ignored for FG_CACHE_SAME */
+  const float* v_scale;
+  int64_t k_scale_batch_stride, k_scale_head_stride; /* elements between sequences / KV heads, 0 where shared */
+  int64_t v_scale_batch_stride, v_scale_head_stride;
+} FgCacheAttnParams;
+
+/* Attention forward for these parameters.  Entries of the block table that lie outside every window are not read.  A
+ * sequence that needs an entry naming no page of the cache, or more entries than a row of the table has, gives NaN.
+ * The reference accepts the descale arguments and ignores them (src/flag_gems/ops/attention.py:1118-1287). */
+int fg_cache_attn_fwd(const FgCacheAttnParams* p /*host*/, void* stream);
+
+/* Scratch the forward would like: partial results of split key ranges.  Without it (NULL or too small) it runs unsplit.
+ * Uninitialised memory is fine; one stream at a time. */
+size_t fg_cache_attn_workspace_bytes(const FgCacheAttnParams* p /*host*/, int device);
 
 /* ------------------------------------------------------------------------------------------------------------
  * Diagnostics.  Not part of the operator interface: nothing above depends on a caller using them, and a binder of

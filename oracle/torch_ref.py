@@ -339,3 +339,87 @@ def decoder_layer(h, wqkv, wo, wgu, wd, n1, n2, positions, cos, sin, eps, heads,
     out = rnd(rnd(act @ wd.t()) + resid)
     return {"x": x, "k": k, "v": v, "q": q, "attn": att, "o": o, "y": y, "residual": resid, "gate_up": gu,
             "act": act, "out": out}
+
+
+# ---- the 8-bit paged cache (no counterpart in the reference, which ignores kv_cache_dtype and the scales): 64-bit ----------
+def round_to_8bit(x, fmt):
+    """x (float64) rounded to the nearest e4m3 / e5m2 value, ties to even, cut to the format's range; NaN stays NaN."""
+    bits, low, top = {"e4m3": (3, -6, 448.0), "e5m2": (2, -14, 57344.0)}[fmt]
+    x = x.double()
+    mag = torch.nan_to_num(x.abs(), nan=0.0, posinf=top).clamp(min=2.0 ** -80)
+    step = torch.exp2(torch.floor(torch.log2(mag)).clamp(min=low) - bits)
+    return (torch.round(x / step) * step).clamp(-top, top)
+
+
+def per_head(scale, heads):
+    """A scale of one number or one for each head as [heads, 1] in float64; None: ones."""
+    if scale is None:
+        return torch.ones(heads, 1, dtype=torch.float64)
+    return to_reference(scale).double().reshape(-1, 1).expand(heads, 1)
+
+
+def cache_write_8bit(key, cache_values, slot_mapping, scale, fmt):
+    """Values (float64) that the cache holds after key / scale was written to its slots."""
+    out = to_reference(cache_values).double().clone()
+    flat = out.view(-1, *out.shape[2:])
+    rows = to_reference(key).double() / per_head(scale, key.shape[1])
+    for i, slot in enumerate(to_reference(slot_mapping).tolist()):
+        if 0 <= slot < flat.shape[0]:
+            flat[slot] = round_to_8bit(rows[i], fmt)
+    return out
+
+
+def cache_attention(q, key_cache, value_cache, cu_seqlens_q, seqused_k, block_table, scale, causal=True, window=(-1, -1),
+                    sinks=0, softcap=0.0, k_scale=None, v_scale=None):
+    """Attention over a paged cache in float64, from the definition.  Query i of a sequence with n new tokens and L keys
+    stands at position P = L - n + i; key j is visible iff j <= P + right (right = 0 if causal) and (j >= P - left or
+    j < sinks).  k_scale / v_scale expand to (batch, kv heads).  Returns a dict: out, lse (rows that see nothing: 0, +inf),
+    and what error bounds need: spread = softmax @ |v| , reach = largest scale * sum |q||k| of a visible key, total = sum of
+    |v| over visible keys, seen = number of visible keys."""
+    q, kc, vc, table = (to_reference(t) for t in (q, key_cache, value_cache, block_table))
+    cu, used = to_reference(cu_seqlens_q).tolist(), to_reference(seqused_k).tolist()
+    _, page, hk, dim = kc.shape
+    total_q, hq, _ = q.shape
+    batch = len(used)
+    left, right = window
+    right = 0 if causal else right
+    expand = lambda s: torch.ones(batch, hk, dtype=torch.float64) if s is None else to_reference(s).double().expand(batch, hk)  # noqa: E731
+    ks, vs = expand(k_scale), expand(v_scale)
+    res = {"out": torch.zeros(total_q, hq, dim, dtype=torch.float64), "lse": torch.full((hq, total_q), float("inf"), dtype=torch.float64),
+           "spread": torch.zeros(total_q, hq, dim, dtype=torch.float64), "total": torch.zeros(total_q, hq, dim, dtype=torch.float64),
+           "reach": torch.zeros(hq, total_q, dtype=torch.float64), "seen": torch.zeros(hq, total_q, dtype=torch.float64)}
+    for b in range(batch):
+        n, length = cu[b + 1] - cu[b], used[b]
+        if n <= 0 or length <= 0:
+            continue
+        pos = torch.arange(length - n, length)[:, None]
+        j = torch.arange(length)[None, :]
+        seen = torch.ones(n, length, dtype=torch.bool)
+        if right >= 0:
+            seen &= j <= pos + right
+        if left >= 0:
+            seen &= (j >= pos - left) | (j < sinks)
+        keys = torch.nonzero(seen.any(0)).flatten()
+        if not len(keys):
+            continue
+        seen = seen[:, keys]
+        blocks = table[b, keys // page].long()
+        k = kc.view(torch.uint8)[blocks, keys % page].view(kc.dtype).float().double() * ks[b][:, None]
+        v = vc.view(torch.uint8)[blocks, keys % page].view(vc.dtype).float().double() * vs[b][:, None]
+        for h in range(hq):
+            kv = h // (hq // hk)
+            qh = q[cu[b]:cu[b + 1], h].double()
+            t = scale * (qh @ k[:, kv].t())
+            if softcap > 0:
+                t = softcap * torch.tanh(t / softcap)
+            t = t.masked_fill(~seen, float("-inf"))
+            some = seen.any(1)
+            rows = torch.arange(cu[b], cu[b + 1])[some]
+            p = torch.softmax(t[some], 1)
+            res["out"][rows, h] = p @ v[:, kv]
+            res["spread"][rows, h] = p @ v[:, kv].abs()
+            res["total"][rows, h] = seen[some].double() @ v[:, kv].abs()
+            res["lse"][h, rows] = torch.logsumexp(t[some], 1)
+            res["reach"][h, rows] = (scale * (qh[some].abs() @ k[:, kv].abs().t())).masked_fill(~seen[some], 0).amax(1)
+            res["seen"][h, rows] = seen[some].double().sum(1)
+    return res
