@@ -1,5 +1,5 @@
 // What the attention kernels over a paged cache share: arguments, the cache's element types, which keys a block of rows sees.
-// Included by attn_cache.hip inside its unnamed namespace, in front of attn_stream.h.
+// Included by attn_cache.hip inside its unnamed namespace, in front of attn_stream.h and attn_tile.h.
 #pragma once
 
 struct CacheAttnArgs {
@@ -13,6 +13,7 @@ struct CacheAttnArgs {
   int min_q, max_q;            // sequences with min_q..max_q new tokens are taken, others are left alone
   uint32_t page_magic;         // page number of key k: (k * page_magic) >> page_shift
   int page_shift;
+  int page_bits;               // log2(page_size) where it is a power of two, else -1
   float* part_o;               // [splits][batch][max_q][Hq][DP] fp32, not divided by the sum   (splits > 1)
   float* part_ml;              // [splits][batch][max_q][Hq][2] fp32: maximum (base 2), sum
 };
@@ -96,4 +97,10 @@ __device__ __forceinline__ void row_bounds(const CacheAttnArgs& a, int q_len, in
   const int64_t h = at + 1 + a.right, l = at - a.left;
   hi = h < k_len ? (h > 0 ? (int)h : 0) : k_len;
   lo = l > 0 ? (l < k_len ? (int)l : k_len) : 0;
+}
+// ds_read_b64_tr_b16: the 16 lanes of a group read four rows of 16 elements; lane i receives element i of the four rows.
+__device__ __forceinline__ u32x2 read_tr(const char* at) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at));
 }

@@ -13,6 +13,7 @@ namespace {
 
 #include "attn_cache.h"
 #include "attn_stream.h"
+#include "attn_tile.h"
 
 template <typename T, int FMT, int DP>
 int stream_rows(const CacheAttnArgs& a, int nq, bool narrow, hipStream_t st) {
@@ -36,6 +37,14 @@ int stream_formats(const CacheAttnArgs& a, int nq, bool narrow, hipStream_t st) 
   return stream_dims<T, FG_CACHE_SAME>(a, nq, narrow, st);
 }
 
+template <typename T>
+int tile_formats(const CacheAttnArgs& a, hipStream_t st) {
+  const bool small = a.p.base.D <= 64;
+  if (a.p.cache_format == FG_CACHE_E4M3) return small ? launch_tile<T, FG_CACHE_E4M3, 64>(a, st) : launch_tile<T, FG_CACHE_E4M3, 128>(a, st);
+  if (a.p.cache_format == FG_CACHE_E5M2) return small ? launch_tile<T, FG_CACHE_E5M2, 64>(a, st) : launch_tile<T, FG_CACHE_E5M2, 128>(a, st);
+  return small ? launch_tile<T, FG_CACHE_SAME, 64>(a, st) : launch_tile<T, FG_CACHE_SAME, 128>(a, st);
+}
+
 int num_cu() {
   int dev = 0, n = 0;
   if (hipGetDevice(&dev) != hipSuccess) dev = 0;
@@ -44,7 +53,8 @@ int num_cu() {
 }
 
 struct Plan {
-  int stream_q;     // most new tokens of a sequence
+  int stream_q;     // sequences with up to so many new tokens take the stream kernel (0: none)
+  bool tile;        // the others take the tile kernel
   int nq;           // stream kernel: 16-row tiles of a row block
   bool narrow;      // stream kernel: pages of a size that is not a multiple of 8
   int splits;       // stream kernel: key ranges
@@ -53,12 +63,16 @@ struct Plan {
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 
-// How the rows and the keys are cut.
+// Which kernels run, and how the rows and the keys are cut.
 Plan make_plan(const FgCacheAttnParams& c) {
   const FgFlashParams& p = c.base;
   const int G = p.Hq / p.Hk;
   Plan plan;
-  plan.stream_q = p.max_seqlen_q;
+  const int few = 32 / G > 1 ? 32 / G : 1;
+  plan.tile = p.D <= 128 && p.max_seqlen_q > few;
+  plan.stream_q = plan.tile ? few : p.max_seqlen_q;
+  // every sequence as long as the longest: the stream kernel has none to take
+  if (plan.tile && (int64_t)p.total_q >= (int64_t)p.batch * p.max_seqlen_q) plan.stream_q = 0;
   plan.narrow = p.page_size % 8 != 0;
   plan.nq = !plan.narrow && p.D <= 128 && (int64_t)plan.stream_q * G > 16 ? 2 : 1;
   // the most keys that one row block may see
@@ -69,7 +83,7 @@ Plan make_plan(const FgCacheAttnParams& c) {
   }
   const int64_t tiles = fg_cdiv(keys, kTile);
   const int64_t row_blocks = fg_cdiv((int64_t)plan.stream_q * G, 16 * plan.nq);
-  const int64_t groups = row_blocks * p.batch * p.Hk;
+  const int64_t groups = (row_blocks > 0 ? row_blocks : 1) * p.batch * p.Hk;
   int64_t splits = fg_cdiv(2 * (int64_t)num_cu(), groups);
   const int64_t most = tiles / 16 > 1 ? tiles / 16 : 1;
   if (splits > most) splits = most;
@@ -135,6 +149,7 @@ extern "C" int fg_cache_attn_fwd(const FgCacheAttnParams* c, void* stream) {
   while (((int64_t)1 << s) < p.page_size) ++s;
   a.page_magic = (uint32_t)(((uint64_t)1 << (31 + s)) / (uint64_t)p.page_size + 1);
   a.page_shift = 31 + s;
+  a.page_bits = ((int64_t)1 << s) == p.page_size ? s : -1;
   const Plan plan = make_plan(*c);
   a.splits = plan.splits;
   if (plan.splits > 1 && (p.workspace == nullptr || (size_t)p.workspace_bytes < plan.workspace || !fg_aligned(p.workspace, 16))) a.splits = 1;
@@ -142,7 +157,13 @@ extern "C" int fg_cache_attn_fwd(const FgCacheAttnParams* c, void* stream) {
   a.part_o = (float*)p.workspace;
   a.part_ml = a.part_o + (size_t)a.splits * p.batch * plan.stream_q * p.Hq * padded_dim(p.D);
   hipStream_t st = (hipStream_t)stream;
-  a.min_q = 1;
-  a.max_q = plan.stream_q;
-  return p.dtype == FG_F16 ? stream_formats<f16_t>(a, plan.nq, plan.narrow, st) : stream_formats<bf16_t>(a, plan.nq, plan.narrow, st);
+  if (plan.stream_q > 0) {
+    a.min_q = 1;
+    a.max_q = plan.stream_q;
+    const int done = p.dtype == FG_F16 ? stream_formats<f16_t>(a, plan.nq, plan.narrow, st) : stream_formats<bf16_t>(a, plan.nq, plan.narrow, st);
+    if (done != FG_OK || !plan.tile) return done;
+  }
+  a.min_q = plan.stream_q + 1;
+  a.max_q = p.max_seqlen_q;
+  return p.dtype == FG_F16 ? tile_formats<f16_t>(a, st) : tile_formats<bf16_t>(a, st);
 }
