@@ -8,14 +8,17 @@ struct CacheAttnArgs {
   float cap_in, cap_out_log2;  // softcap: t = cap_out_log2 * tanh(S * cap_in)
   int group;                   // query heads per KV head
   int left, right;             // window bounds, INT32_MAX where unbounded
-  int splits;                  // key ranges per row block (grid x = splits * row blocks)
-  int min_tiles;               // fewest tiles of a range, a multiple of 4
+  int splits;                  // key ranges per row block
+  int min_tiles;               // fewest tiles of a range
   int min_q, max_q;            // sequences with min_q..max_q new tokens are taken, others are left alone
   uint32_t page_magic;         // page number of key k: (k * page_magic) >> page_shift
   int page_shift;
   int page_bits;               // log2(page_size) where it is a power of two, else -1
-  float* part_o;               // [splits][batch][max_q][Hq][DP] fp32, not divided by the sum   (splits > 1)
-  float* part_ml;              // [splits][batch][max_q][Hq][2] fp32: maximum (base 2), sum
+  // splits > 1: partial results, fp32.  Rows are tokens: part_q of each sequence, or all tokens of the call (part_q == 0)
+  int part_q;
+  int64_t part_rows;           // batch * part_q, or total_q
+  float* part_o;               // [splits][part_rows][Hq][DP], not divided by the sum
+  float* part_ml;              // [splits][part_rows][Hq][2]: maximum (base 2), sum
 };
 
 // ---- element types of the cache ------------------------------------------------------------------------------------------
@@ -98,9 +101,166 @@ __device__ __forceinline__ void row_bounds(const CacheAttnArgs& a, int q_len, in
   hi = h < k_len ? (h > 0 ? (int)h : 0) : k_len;
   lo = l > 0 ? (l < k_len ? (int)l : k_len) : 0;
 }
+// A sequence as a workgroup takes it; `mine` is false where it is not for this launch.
+struct Sequence {
+  int q_bos, q_len, k_len;
+  float k_scale, v_scale;
+  bool mine, too_long;  // longer than its row of the block table: nothing is read behind the row, its output is NaN
+};
+// Everything that does not depend on other loads is requested at once: each trip to memory is about a microsecond, and a
+// short call is little else.
+__device__ __forceinline__ Sequence sequence(const CacheAttnArgs& a, int b, int kvh) {
+  const FgFlashParams& p = a.p.base;
+  Sequence s;
+  const int end = p.cu_seqlens_q[b + 1];
+  const int k_said = p.seqused_k[b];
+  s.q_bos = p.cu_seqlens_q[b];
+  s.k_scale = seq_scale(a.p.k_scale, a.p.k_scale_batch_stride, a.p.k_scale_head_stride, b, kvh);
+  s.v_scale = seq_scale(a.p.v_scale, a.p.v_scale_batch_stride, a.p.v_scale_head_stride, b, kvh);
+  s.q_len = end - s.q_bos;
+  s.mine = s.q_len >= a.min_q && s.q_len <= a.max_q && s.q_bos >= 0 && end <= p.total_q;
+  const int64_t reach = (int64_t)a.p.table_width * p.page_size;
+  s.too_long = k_said > reach;
+  s.k_len = k_said < 0 ? 0 : (k_said < reach ? k_said : (int)reach);
+  return s;
+}
+// tanh to about 4 roundings: its series near 0, (1 - e) / (1 + e) with e = exp(-2x) elsewhere.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float ax = fabsf(x), x2 = x * x;
+  const float near0 = x + x * x2 * (-1.f / 3 + x2 * (2.f / 15 + x2 * (-17.f / 315 + x2 * (62.f / 2835))));
+  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(ax * 2.8853900817779268f));
+  return ax < 0.25f ? near0 : copysignf(far, x);
+}
+// In every 16 lanes: lanes 8-15 of `lo` and lanes 0-7 of `hi` change places.
+__device__ __forceinline__ void swap_half_rows(uint32_t& lo, uint32_t& hi) {
+  constexpr int kRor8 = 0x128;  // the lane 8 further on, round the 16
+  const int a = (int)lo, b = (int)hi;
+  lo = (uint32_t)__builtin_amdgcn_update_dpp(a, b, kRor8, 0xF, 0xC, false);
+  hi = (uint32_t)__builtin_amdgcn_update_dpp(b, a, kRor8, 0xF, 0x3, false);
+}
 // ds_read_b64_tr_b16: the 16 lanes of a group read four rows of 16 elements; lane i receives element i of the four rows.
 __device__ __forceinline__ u32x2 read_tr(const char* at) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4* lds_ptr;
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at));
+}
+
+// ---- key ranges ----------------------------------------------------------------------------------------------------------
+// A row block's tiles are spread over all `splits` ranges, whatever the host knew of the sequence's length, but a range has at
+// least min_tiles of them, and a multiple of UNIT.
+template <int UNIT>
+__device__ __forceinline__ int range_tiles(const CacheAttnArgs& a, int tiles) {
+  const int t = ((tiles + a.splits - 1) / a.splits + UNIT - 1) / UNIT * UNIT;
+  return t < a.min_tiles && a.splits > 1 ? a.min_tiles : t;
+}
+__device__ __forceinline__ int64_t part_row(const CacheAttnArgs& a, int split, int b, int q_bos, int tok) {
+  return split * a.part_rows + (a.part_q > 0 ? (int64_t)b * a.part_q : q_bos) + tok;
+}
+
+// Merges the key ranges of a row (token, head), which belongs to a block of ROWS rows whose tiles have TILE keys.  WHOLE: a
+// workgroup for each row (many ranges), else a wave.  A lane holds four elements; what lanes are left take other ranges.
+template <typename T, int DP, int TILE, int ROWS, int UNIT, bool WHOLE>
+__global__ __launch_bounds__(256) void attn_merge_kernel(CacheAttnArgs a) {
+  constexpr int LR = DP / 4;                     // lanes of a row
+  constexpr int NG = (WHOLE ? 256 : 64) / LR;    // groups of ranges
+  __shared__ __attribute__((aligned(16))) float parts[WHOLE ? 4 : 1][DP + 4];
+  const FgFlashParams& p = a.p.base;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t th = WHOLE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;  // token * Hq + head
+  const int b = blockIdx.y;
+  const int tok = (int)(th / p.Hq), head = (int)(th - (int64_t)tok * p.Hq);
+  const Sequence seq = sequence(a, b, head / a.group);
+  const int q_bos = seq.q_bos, q_len = seq.q_len, k_len = seq.k_len;
+  if (!seq.mine || tok >= q_len) return;         // (the same for all threads of a row)
+  const int rows = q_len * a.group;
+  const int row0 = (tok * a.group + head % a.group) / ROWS * ROWS;
+  const int last_row = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
+  const Seen seen = seen_by<TILE>(a, q_len, k_len, row0 / a.group, last_row / a.group);
+  const int per = range_tiles<UNIT>(a, seen.tiles);
+  int ns = per > 0 ? (seen.tiles + per - 1) / per : 1;  // ranges that were written
+  ns = ns < 1 ? 1 : (ns > a.splits ? a.splits : ns);
+  const int64_t step = a.part_rows * p.Hq, at = part_row(a, 0, b, q_bos, tok) * p.Hq + head;
+  // a lane's own ranges, four at a time, under their running maximum
+  const int mine = (WHOLE ? tid : lane) / LR, d = (tid % LR) * 4;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f, m = -INFINITY;
+  for (int s0 = mine; s0 < ns; s0 += 4 * NG) {
+    f32x2 ml[4];
+    f32x4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                // (a range past the last one: the last one, with no weight)
+      const int s = s0 + i * NG < ns ? s0 + i * NG : ns - 1;
+      ml[i] = *reinterpret_cast<const f32x2*>(a.part_ml + (s * step + at) * 2);
+      x[i] = *reinterpret_cast<const f32x4*>(a.part_o + (s * step + at) * DP + d);
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i][0]);
+    const float use = top == -INFINITY ? 0.f : top;
+    const float old = __builtin_amdgcn_exp2f(m - use);
+    l *= old;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= old;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s0 + i * NG >= ns) continue;
+      const float f = __builtin_amdgcn_exp2f(ml[i][0] - use);
+      l += ml[i][1] * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += x[i][e] * f;
+    }
+    m = top;
+  }
+  // the groups of a wave, then the waves
+  float all = m;
+#pragma unroll
+  for (int x = LR; x < 64; x *= 2) all = fmaxf(all, __shfl_xor(all, x, 64));
+  float m_use = all == -INFINITY ? 0.f : all;
+  const float own = __builtin_amdgcn_exp2f(m - m_use);
+  l *= own;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= own;
+#pragma unroll
+  for (int x = LR; x < 64; x *= 2) {
+    l += __shfl_xor(l, x, 64);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x, 64);
+  }
+  if constexpr (WHOLE) {
+    if (lane < LR) *reinterpret_cast<f32x4*>(&parts[wave][d]) = o;
+    if (lane == 0) parts[wave][DP] = l, parts[wave][DP + 1] = all;
+    __syncthreads();
+    if (tid >= LR) return;
+    all = fmaxf(fmaxf(parts[0][DP + 1], parts[1][DP + 1]), fmaxf(parts[2][DP + 1], parts[3][DP + 1]));
+    m_use = all == -INFINITY ? 0.f : all;
+    o = f32x4{0.f, 0.f, 0.f, 0.f}, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(parts[w][DP + 1] - m_use);
+      l += parts[w][DP] * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += parts[w][d + e] * f;
+    }
+  } else if (lane >= LR) {
+    return;
+  }
+  const bool empty = l == 0.f;
+  const float f = empty ? 0.f : seq.v_scale / l;
+  T* const out = (T*)p.out + (int64_t)(q_bos + tok) * p.o_row_stride + (int64_t)head * p.o_head_stride;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (d + e < p.D) out[d + e] = (T)(empty ? 0.f : o[e] * f);
+  if (d == 0 && p.lse != nullptr)
+    p.lse[(int64_t)head * p.total_q + q_bos + tok] = empty ? INFINITY : m_use * 0.6931471805599453f + logf(l);
+}
+
+template <typename T, int DP, int TILE, int ROWS, int UNIT>
+int launch_merge(const CacheAttnArgs& a, hipStream_t st) {
+  const FgFlashParams& p = a.p.base;
+  const int64_t rows = (int64_t)a.max_q * p.Hq;
+  if (a.splits > 8)
+    hipLaunchKernelGGL((attn_merge_kernel<T, DP, TILE, ROWS, UNIT, true>), dim3((unsigned)rows, (unsigned)p.batch), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((attn_merge_kernel<T, DP, TILE, ROWS, UNIT, false>), dim3((unsigned)fg_cdiv(rows, 4), (unsigned)p.batch), dim3(256), 0, st, a);
+  return fg_check_launch("cache_attn_fwd");
 }

@@ -7,6 +7,8 @@
 //
 // c, c' are the cached K and V values as they stand, s the scales they were written with (1 for a 16-bit cache).
 #include <limits.h>
+#include <algorithm>
+#include <atomic>
 #include "fg_common.h"
 
 namespace {
@@ -16,79 +18,135 @@ namespace {
 #include "attn_tile.h"
 
 template <typename T, int FMT, int DP>
-int stream_rows(const CacheAttnArgs& a, int nq, bool narrow, hipStream_t st) {
-  if (narrow) return launch_stream<T, FMT, DP, 1, true>(a, st);
+int stream_pages(const CacheAttnArgs& a, int nq, int pages, hipStream_t st) {
+  if (pages == kKeys) return launch_stream<T, FMT, DP, 1, kKeys>(a, st);
   if constexpr (DP < 256) {
-    if (nq == 2) return launch_stream<T, FMT, DP, 2, false>(a, st);
+    if (nq == 2) return pages == kHalves ? launch_stream<T, FMT, DP, 2, kHalves>(a, st) : launch_stream<T, FMT, DP, 2, kGroups>(a, st);
   }
-  return launch_stream<T, FMT, DP, 1, false>(a, st);
+  return pages == kHalves ? launch_stream<T, FMT, DP, 1, kHalves>(a, st) : launch_stream<T, FMT, DP, 1, kGroups>(a, st);
 }
 template <typename T, int FMT>
-int stream_dims(const CacheAttnArgs& a, int nq, bool narrow, hipStream_t st) {
+int stream_dims(const CacheAttnArgs& a, int nq, int pages, hipStream_t st) {
   const int D = a.p.base.D;
-  if (D <= 64) return stream_rows<T, FMT, 64>(a, nq, narrow, st);
-  if (D <= 128) return stream_rows<T, FMT, 128>(a, nq, narrow, st);
-  return stream_rows<T, FMT, 256>(a, nq, narrow, st);
+  if (D <= 64) return stream_pages<T, FMT, 64>(a, nq, pages, st);
+  if (D <= 128) return stream_pages<T, FMT, 128>(a, nq, pages, st);
+  return stream_pages<T, FMT, 256>(a, nq, pages, st);
 }
 template <typename T>
-int stream_formats(const CacheAttnArgs& a, int nq, bool narrow, hipStream_t st) {
-  if (a.p.cache_format == FG_CACHE_E4M3) return stream_dims<T, FG_CACHE_E4M3>(a, nq, narrow, st);
-  if (a.p.cache_format == FG_CACHE_E5M2) return stream_dims<T, FG_CACHE_E5M2>(a, nq, narrow, st);
-  return stream_dims<T, FG_CACHE_SAME>(a, nq, narrow, st);
+int stream_formats(const CacheAttnArgs& a, int nq, int pages, hipStream_t st) {
+  if (a.p.cache_format == FG_CACHE_E4M3) return stream_dims<T, FG_CACHE_E4M3>(a, nq, pages, st);
+  if (a.p.cache_format == FG_CACHE_E5M2) return stream_dims<T, FG_CACHE_E5M2>(a, nq, pages, st);
+  return stream_dims<T, FG_CACHE_SAME>(a, nq, pages, st);
 }
 
+template <typename T, int FMT>
+int tile_dims(const CacheAttnArgs& a, int nq, hipStream_t st) {
+  if (a.p.base.D <= 64) return nq == 1 ? launch_tile<T, FMT, 64, 1>(a, st) : launch_tile<T, FMT, 64, 2>(a, st);
+  return nq == 1 ? launch_tile<T, FMT, 128, 1>(a, st) : launch_tile<T, FMT, 128, 2>(a, st);
+}
 template <typename T>
-int tile_formats(const CacheAttnArgs& a, hipStream_t st) {
-  const bool small = a.p.base.D <= 64;
-  if (a.p.cache_format == FG_CACHE_E4M3) return small ? launch_tile<T, FG_CACHE_E4M3, 64>(a, st) : launch_tile<T, FG_CACHE_E4M3, 128>(a, st);
-  if (a.p.cache_format == FG_CACHE_E5M2) return small ? launch_tile<T, FG_CACHE_E5M2, 64>(a, st) : launch_tile<T, FG_CACHE_E5M2, 128>(a, st);
-  return small ? launch_tile<T, FG_CACHE_SAME, 64>(a, st) : launch_tile<T, FG_CACHE_SAME, 128>(a, st);
+int tile_formats(const CacheAttnArgs& a, int nq, hipStream_t st) {
+  if (a.p.cache_format == FG_CACHE_E4M3) return tile_dims<T, FG_CACHE_E4M3>(a, nq, st);
+  if (a.p.cache_format == FG_CACHE_E5M2) return tile_dims<T, FG_CACHE_E5M2>(a, nq, st);
+  return tile_dims<T, FG_CACHE_SAME>(a, nq, st);
 }
 
 int num_cu() {
+  static std::atomic<int> known[64];             // by device; two queries of the runtime a call otherwise
   int dev = 0, n = 0;
   if (hipGetDevice(&dev) != hipSuccess) dev = 0;
+  if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+  if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
 struct Plan {
   int stream_q;     // sequences with up to so many new tokens take the stream kernel (0: none)
   bool tile;        // the others take the tile kernel
-  int nq;           // stream kernel: 16-row tiles of a row block
-  bool narrow;      // stream kernel: pages of a size that is not a multiple of 8
-  int splits;       // stream kernel: key ranges
-  size_t workspace;
+  int nq, tile_nq;  // 16-row tiles of a row block (stream), of a wave (tile)
+  int pages;        // stream kernel: how pages are found
+  int splits, min_tiles, tile_splits, tile_min_tiles;
+  size_t stream_bytes, tile_bytes;  // scratch for the key ranges; one after the other
 };
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
+
+// Microseconds that a launch of the tile kernel takes with row blocks of 64 * nq rows and `splits` key ranges, from what was
+// measured on MI355X: the steps of a tile on a CU that holds one workgroup or two, start and end of a workgroup, and the merge
+// (its launch, and 2 * (DP + 2) * 4 bytes for each range, token and head at 5 TB/s).  `even`: all sequences as long as the
+// longest; otherwise their blocks are taken to be 0.6 of the longest on average, and a long one to begin among the last.  Chunks
+// of (1024, 765, 284, 14) tokens over (8192, 4816, 3212, 2548) keys, 32/8 heads: 577 us unsplit, 306 in 2 ranges, 312 in 4 (308
+// here), 516 in 12; one chunk of 1000 over 1000: blocks of 64 rows 35 us, of 128 rows 43, in 2 ranges 53 and 55.
+double tile_cost(int64_t blocks, double tiles, int nq, int dp, int64_t cus, int splits, bool even, double merge_bytes) {
+  const double dim = dp == 64 ? 0.72 : 1.0;
+  const double alone = (nq == 1 ? 1.32 : 1.7) * dim, shared = (nq == 1 ? 1.54 : 2.3) * dim;
+  const int64_t wgs = blocks * splits;
+  const double range = tiles / splits < 1 ? 1 : tiles / splits;
+  double us = 6;
+  if (wgs <= cus) us += range * alone;
+  else if (wgs <= 2 * cus) us += range * shared;
+  else if (even) us += (double)fg_cdiv(wgs, 2 * cus) * range * shared;
+  else us += (0.6 * (double)blocks * tiles / (double)(2 * cus) + 0.75 * range) * shared;
+  if (splits > 1) us += 4 + splits * merge_bytes * 2 / 5e6;
+  return us;
+}
 
 // Which kernels run, and how the rows and the keys are cut.
 Plan make_plan(const FgCacheAttnParams& c) {
   const FgFlashParams& p = c.base;
   const int G = p.Hq / p.Hk;
-  Plan plan;
+  const int64_t cus = num_cu();
+  Plan plan = {};
   const int few = 32 / G > 1 ? 32 / G : 1;
   plan.tile = p.D <= 128 && p.max_seqlen_q > few;
   plan.stream_q = plan.tile ? few : p.max_seqlen_q;
   // every sequence as long as the longest: the stream kernel has none to take
   if (plan.tile && (int64_t)p.total_q >= (int64_t)p.batch * p.max_seqlen_q) plan.stream_q = 0;
-  plan.narrow = p.page_size % 8 != 0;
-  plan.nq = !plan.narrow && p.D <= 128 && (int64_t)plan.stream_q * G > 16 ? 2 : 1;
-  // the most keys that one row block may see
-  int64_t keys = p.max_seqlen_k > 0 ? p.max_seqlen_k : 1;
-  if (p.window_left >= 0) {
-    const int64_t window = (int64_t)p.window_left + plan.stream_q + c.num_sink_tokens + 2 * kTile;
-    keys = window < keys ? window : keys;
+  const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
+  plan.pages = pow2 && p.page_size >= 16 ? kHalves : (p.page_size % 8 == 0 ? kGroups : kKeys);
+  plan.nq = plan.pages != kKeys && p.D <= 128 && (int64_t)plan.stream_q * G > 16 ? 2 : 1;
+  // the most keys that one row block of `q` tokens may see
+  auto keys_of = [&](int64_t q, int tile) {
+    int64_t keys = p.max_seqlen_k > 0 ? p.max_seqlen_k : 1;
+    const int64_t window = (int64_t)p.window_left + q + c.num_sink_tokens + 2 * tile;
+    return p.window_left >= 0 && window < keys ? window : keys;
+  };
+  const size_t row = (size_t)p.Hq * (padded_dim(p.D) + 2) * sizeof(float);
+  plan.splits = 1;
+  if (plan.stream_q > 0) {
+    const int64_t tiles = fg_cdiv(keys_of(fg_cdiv(16 * plan.nq, G), kTile), kTile);
+    const int64_t groups = fg_cdiv((int64_t)plan.stream_q * G, 16 * plan.nq) * p.batch * p.Hk;
+    // Two workgroups per CU fill the card.  Below that the keys are cut into ranges for up to four per CU (sequences differ, and
+    // the ranges of a short one end early) of at least 16 tiles, or for one per CU of at least 4: 24 groups of 4096 tiles take
+    // 1400 us unsplit, 138 cut in 16 and 115 in 43; 8 groups of 62 tiles 21 us unsplit, 13 cut in 12; 512 groups of 128 tiles
+    // 105 us unsplit, 108 cut in 3.  Up to 32 tiles the launch that merges costs what the ranges save.
+    plan.min_tiles = 4;
+    int64_t splits = 1;
+    if (groups < 2 * cus && tiles > 32) {
+      const int64_t many = std::min(fg_cdiv(4 * cus, groups), tiles / 16), few_keys = std::min(fg_cdiv(cus, groups), tiles / 4);
+      splits = std::max(std::max(many, few_keys), (int64_t)1);
+    }
+    plan.splits = (int)splits;
+    if (plan.splits > 1) plan.stream_bytes = (plan.splits * row * p.batch * plan.stream_q + 15) / 16 * 16;
   }
-  const int64_t tiles = fg_cdiv(keys, kTile);
-  const int64_t row_blocks = fg_cdiv((int64_t)plan.stream_q * G, 16 * plan.nq);
-  const int64_t groups = (row_blocks > 0 ? row_blocks : 1) * p.batch * p.Hk;
-  int64_t splits = fg_cdiv(2 * (int64_t)num_cu(), groups);
-  const int64_t most = tiles / 16 > 1 ? tiles / 16 : 1;
-  if (splits > most) splits = most;
-  plan.splits = (int)splits;
-  plan.workspace = splits > 1 ? (size_t)splits * p.batch * plan.stream_q * p.Hq * (padded_dim(p.D) + 2) * sizeof(float) : 0;
+  if (plan.tile) {
+    const bool even = plan.stream_q == 0;
+    const int dp = padded_dim(p.D);
+    double best = 0;
+    for (int nq = 1; nq <= 2; ++nq) {
+      const int rows = 64 * nq;
+      // even: exact; otherwise half a block is left over in a sequence on average
+      const int64_t blocks = p.Hk * (even ? fg_cdiv((int64_t)p.max_seqlen_q * G, rows) * p.batch : (int64_t)p.total_q * G / rows + p.batch / 2 + 1);
+      const int64_t tiles = fg_cdiv(keys_of(fg_cdiv(rows, G), kTileKeys), kTileKeys);
+      for (int splits = 1; splits <= 64 && (splits == 1 || tiles >= 2 * splits); ++splits) {
+        const double us = tile_cost(blocks, (double)tiles, nq, dp, cus, splits, even, (double)row * (double)p.total_q);
+        if (plan.tile_splits == 0 || us < best) best = us, plan.tile_nq = nq, plan.tile_splits = splits;
+      }
+    }
+    plan.tile_min_tiles = 2;
+    if (plan.tile_splits > 1) plan.tile_bytes = plan.tile_splits * row * p.total_q;
+  }
   return plan;
 }
 
@@ -127,7 +185,8 @@ int check_params(const FgCacheAttnParams* c) {
 extern "C" size_t fg_cache_attn_workspace_bytes(const FgCacheAttnParams* c, int device) {
   (void)device;
   if (c == nullptr || c->base.batch <= 0 || c->base.total_q <= 0 || check_params(c) != FG_OK) return 0;
-  return make_plan(*c).workspace;
+  const Plan plan = make_plan(*c);
+  return plan.stream_bytes + plan.tile_bytes;
 }
 
 extern "C" int fg_cache_attn_fwd(const FgCacheAttnParams* c, void* stream) {
@@ -151,19 +210,28 @@ extern "C" int fg_cache_attn_fwd(const FgCacheAttnParams* c, void* stream) {
   a.page_shift = 31 + s;
   a.page_bits = ((int64_t)1 << s) == p.page_size ? s : -1;
   const Plan plan = make_plan(*c);
-  a.splits = plan.splits;
-  if (plan.splits > 1 && (p.workspace == nullptr || (size_t)p.workspace_bytes < plan.workspace || !fg_aligned(p.workspace, 16))) a.splits = 1;
-  a.min_tiles = 16;
-  a.part_o = (float*)p.workspace;
-  a.part_ml = a.part_o + (size_t)a.splits * p.batch * plan.stream_q * p.Hq * padded_dim(p.D);
+  const bool scratch = p.workspace != nullptr && fg_aligned(p.workspace, 16) && (size_t)p.workspace_bytes >= plan.stream_bytes + plan.tile_bytes;
+  const int dp = padded_dim(p.D);
   hipStream_t st = (hipStream_t)stream;
   if (plan.stream_q > 0) {
     a.min_q = 1;
     a.max_q = plan.stream_q;
-    const int done = p.dtype == FG_F16 ? stream_formats<f16_t>(a, plan.nq, plan.narrow, st) : stream_formats<bf16_t>(a, plan.nq, plan.narrow, st);
+    a.splits = scratch ? plan.splits : 1;
+    a.min_tiles = plan.min_tiles;
+    a.part_q = plan.stream_q;
+    a.part_rows = (int64_t)p.batch * plan.stream_q;
+    a.part_o = (float*)p.workspace;
+    a.part_ml = a.part_o + (size_t)a.splits * a.part_rows * p.Hq * dp;
+    const int done = p.dtype == FG_F16 ? stream_formats<f16_t>(a, plan.nq, plan.pages, st) : stream_formats<bf16_t>(a, plan.nq, plan.pages, st);
     if (done != FG_OK || !plan.tile) return done;
   }
   a.min_q = plan.stream_q + 1;
   a.max_q = p.max_seqlen_q;
-  return p.dtype == FG_F16 ? tile_formats<f16_t>(a, st) : tile_formats<bf16_t>(a, st);
+  a.splits = scratch ? plan.tile_splits : 1;
+  a.min_tiles = plan.tile_min_tiles;
+  a.part_q = 0;
+  a.part_rows = p.total_q;
+  a.part_o = (float*)((char*)p.workspace + plan.stream_bytes);
+  a.part_ml = a.part_o + (size_t)a.splits * a.part_rows * p.Hq * dp;
+  return p.dtype == FG_F16 ? tile_formats<f16_t>(a, plan.tile_nq, st) : tile_formats<bf16_t>(a, plan.tile_nq, st);
 }

@@ -18,7 +18,7 @@
 //   K: MFMA row m of half tile t is key (m / 4) * 8 + t * 4 + m % 4, so the accumulators of lane (r, g) are the scores of
 //      keys g * 8 + 0..7: exactly the k-slots that lane supplies to the second product.  P never moves between lanes.
 //   V: lane (i, g) loads, for keys g * 8 + 0..7, the same VC = DP / 16 consecutive elements d = i * VC + j.  An 8 x VC
-//      transpose inside the lane (v_perm) makes fragment j: keys g * 8 + 0..7 of element i * VC + j.  Output sub-tile j
+//      transpose inside the lane (v_perm, in front of the widening) makes fragment j: keys g * 8 + 0..7 of element i * VC + j.  Output sub-tile j
 //      then holds elements j, VC + j, 2 VC + j, ...: a permutation that the epilogue undoes for free, since a lane ends
 //      with consecutive elements.
 // 8-bit caches: v_cvt_scalef32_pk_{bf16,f16}_{fp8,bf8} widens two elements at a time; every e4m3 and e5m2 value is exact in
@@ -36,14 +36,14 @@
 
 constexpr int kTile = 32;  // keys per tile
 
-// Tiles per key range: the tiles spread over all ranges, a multiple of the four waves, at least min_tiles.
-__device__ __forceinline__ int range_tiles(const CacheAttnArgs& a, int tiles) {
-  int t = ((tiles + a.splits - 1) / a.splits + 3) & ~3;
-  return t < a.min_tiles && a.splits > 1 ? a.min_tiles : t;
-}
+// How a wave finds the pages of a tile.
+enum {
+  kHalves,  // power-of-two pages of at least 16 keys: half a tile lies in one page; table entries and page addresses are scalar
+  kGroups,  // pages of a multiple of 8 keys: a lane looks up its group of 8 keys
+  kKeys,    // any page size: a lane looks up each of its keys
+};
 
-// NARROW: pages of a size that is not a multiple of 8 keys (every key looks its page up).
-template <typename T, int FMT, int DP, int NQ, bool NARROW>
+template <typename T, int FMT, int DP, int NQ, int PAGES>
 __global__ __launch_bounds__(256, 2) void attn_stream_kernel(CacheAttnArgs a) {
   typedef typename Mma16<T>::Frag Frag;
   constexpr bool WIDE = FMT == FG_CACHE_SAME;    // the cache holds T
@@ -58,6 +58,11 @@ __global__ __launch_bounds__(256, 2) void attn_stream_kernel(CacheAttnArgs a) {
   constexpr bool LATE = WIDE && DP == 256;
   constexpr int VP = LATE ? 2 : 1;             // parts of a value row
   constexpr int VWP = VW / VP;                   // words of a part
+  // tiles in flight per wave: two where the registers of a wave (256 at two waves per SIMD) hold them
+  constexpr int NB = DP == 256 || (DP == 128 && (WIDE || NQ == 2)) ? 1 : 2;
+  // Loads that take whole 128-byte lines, eight rows at a time: one lane bit then says which piece of the row the lane holds
+  // where the fragment wants it to say which row, and the two loads of a pair exchange halves (swap_half_rows).
+  constexpr bool SWAP_K = KL >= 2, SWAP_V = VW <= 2;
   constexpr int R = 16 * NQ;
   constexpr int EH = DP == 256 ? 2 : 4;          // accumulator elements merged at once
   constexpr int MD = 16 * VC * EH / 4;           // row elements merged at once: DP, or half of 256
@@ -75,41 +80,43 @@ __global__ __launch_bounds__(256, 2) void attn_stream_kernel(CacheAttnArgs a) {
   const int split = (int)((blockIdx.x + (unsigned)(b * 5 + kvh * 3)) % (unsigned)a.splits);
   const int row0 = (int)(blockIdx.x / (unsigned)a.splits) * R;
 
-  const int q_bos = p.cu_seqlens_q[b];
-  const int q_len = p.cu_seqlens_q[b + 1] - q_bos;
+  const Sequence seq = sequence(a, b, kvh);
+  const int q_bos = seq.q_bos, q_len = seq.q_len, k_len = seq.k_len;
   const int rows = q_len * G;
-  if (q_len < a.min_q || q_len > a.max_q || row0 >= rows) return;
-  if (q_bos < 0 || (int64_t)q_bos + q_len > p.total_q) return;
-  // a sequence longer than its row of the block table: nothing is read behind the row, its output is NaN
-  const int64_t reach = (int64_t)a.p.table_width * p.page_size;
-  const int k_said = p.seqused_k[b];
-  const int k_len = k_said < 0 ? 0 : (k_said < reach ? k_said : (int)reach);
+  if (!seq.mine || row0 >= rows) return;
   const int last_row = row0 + R < rows ? row0 + R - 1 : rows - 1;
   const Seen seen = seen_by<kTile>(a, q_len, k_len, row0 / G, last_row / G);
-  const int per = range_tiles(a, seen.tiles);
+  const int per = range_tiles<4>(a, seen.tiles);
   const int t_begin = split * per;
   const int t_end = t_begin + per < seen.tiles ? t_begin + per : seen.tiles;
   if (split > 0 && t_begin >= t_end) return;     // range 0 always reports
 
   // ---- query rows: lane (r, g), step s holds elements of the same place as the key fragments below ------------------------
+  // t = sc * S with sc > 0, so that the largest t is sc times the largest S: the sign goes into the query (0: a query of 0)
+  const bool capped = p.softcap > 0.f;
+  const float given = (capped ? a.cap_in : a.scale_log2) * seq.k_scale;
+  const uint32_t q_keep = given == 0.f ? 0u : ~0u, q_flip = given < 0.f ? 0x80008000u : 0u;
+  const float inner = given == 0.f ? 1.0f : fabsf(given);
+  const float sc = capped ? a.cap_out_log2 : inner;  // of S, or of tanh(inner * S)
   int lo_r[NQ], hi_r[NQ];                        // keys the lane's row sees: [lo_r, hi_r) and [0, min(sinks, hi_r))
-  Frag qf[NQ][KS];
+  u32x4 q_raw[NQ][KS];
+  uint32_t q_mask[NQ];
   const int D = p.D;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int row = row0 + n * 16 + rl;
     const bool ok = row < rows;
+    q_mask[n] = ok ? q_keep : 0u;
     const int tok = (ok ? row : row0) / G, head = kvh * G + (ok ? row : row0) % G;
     row_bounds(a, q_len, k_len, tok, lo_r[n], hi_r[n]);
     const T* q = (const T*)p.q + (int64_t)(q_bos + tok) * p.q_row_stride + (int64_t)head * p.q_head_stride;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = WIDE ? s * 32 + g * 8 : (s >> 1) * 64 + g * 16 + (s & 1) * 8;
-      u32x4 v = {0u, 0u, 0u, 0u};
-      if (ok && d < D) v = *reinterpret_cast<const u32x4*>(q + d);
-      qf[n][s] = __builtin_bit_cast(Frag, v);
+      q_raw[n][s] = *reinterpret_cast<const u32x4*>(q + (d < D ? d : 0));  // (made a fragment behind the first tile's loads)
     }
   }
+  auto q_inside = [&](int s) { return (WIDE ? s * 32 + g * 8 : (s >> 1) * 64 + g * 16 + (s & 1) * 8) < D; };
   f32x4 acc[NQ][VC];
   float m_run[NQ], l_run[NQ];
 #pragma unroll
@@ -119,19 +126,16 @@ __global__ __launch_bounds__(256, 2) void attn_stream_kernel(CacheAttnArgs a) {
     for (int j = 0; j < VC; ++j) acc[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const float k_scale = seq_scale(a.p.k_scale, a.p.k_scale_batch_stride, a.p.k_scale_head_stride, b, kvh);
-  const float sc = a.scale_log2 * k_scale, cap_in = a.cap_in * k_scale;
-  const bool capped = p.softcap > 0.f;
   const char* const kbase = (const char*)p.k_cache + (int64_t)kvh * p.k_head_stride * EB;
   const char* const vbase = (const char*)p.v_cache + (int64_t)kvh * p.v_head_stride * EB;
   const int32_t* const table = p.block_table + (int64_t)b * p.block_table_stride;
-  bool bad = k_said > reach;                     // or a page that the cache does not have was asked for
+  bool bad = seq.too_long, bad_half = false;     // or a page that the cache does not have was asked for
 
   // a key that some row of the block sees
-  auto any_sees = [&](int key) { return key < seen.hi && (key >= seen.lo || key < seen.sinks); };
+  auto any_sees = [&](int key) { return (key < seen.hi) & ((key >= seen.lo) | (key < seen.sinks)); };
   // the group of 8 keys that starts at `key`, or one that is seen where none of them is
   auto usable = [&](int key) {
-    const bool some = key < seen.hi && (key + 8 > seen.lo || key < seen.sinks);
+    const bool some = (key < seen.hi) & ((key + 8 > seen.lo) | (key < seen.sinks));
     return some ? key : (seen.hi - 1) & ~7;
   };
   auto checked = [&](int page) {
@@ -140,89 +144,140 @@ __global__ __launch_bounds__(256, 2) void attn_stream_kernel(CacheAttnArgs a) {
     return ok ? page : 0;
   };
 
-  u32x4 xk[2][KL];                               // the wave's tile
-  uint32_t xv[8][VWP];
-  const int kg = rl >> 2;                        // K: the lane's group of 8 keys
+  u32x4 xk[NB][2][KL];                           // the wave's tiles, as loaded
+  uint32_t xv[NB][8][VWP];
+  // the group of 8 keys of the lane's MFMA row (SWAP_K: of its row in the first load of a pair; in the second, two further)
+  const int kg = SWAP_K ? (rl >> 2) & 1 : rl >> 2;
   // byte offsets of the lane's pieces inside a row; pieces past the head dim read the row's start (K: zeroed, V: not stored)
   int k_at[KL];
 #pragma unroll
   for (int c = 0; c < KL; ++c) {
-    const int d = (c * 4 + g) * EPL;
+    const int d = SWAP_K ? (((c & ~1) + ((rl >> 3) & 1)) * 4 + g) * EPL : (c * 4 + g) * EPL;
     k_at[c] = d < D ? d * EB : 0;
   }
   const bool ragged = D < DP;
-  const int v_at = rl * VC < D ? rl * VC * EB : 0;
-  const int v_second = rl * VC + 8 < D ? 16 : 0;  // second part of a value row, where it lies inside the row
-
-  auto load_words = [](uint32_t (&dst)[VWP], const char* src) {
-    if constexpr (VWP == 1) {
-      dst[0] = __builtin_nontemporal_load((const uint32_t*)src);
-    } else if constexpr (VWP == 2) {
-      const u32x2 w = __builtin_nontemporal_load((const u32x2*)src);
-      dst[0] = w[0], dst[1] = w[1];
-    } else {
-      const u32x4 w = __builtin_nontemporal_load((const u32x4*)src);
-      dst[0] = w[0], dst[1] = w[1], dst[2] = w[2], dst[3] = w[3];
-    }
-  };
+  const int v_first = SWAP_V ? (rl & 7) * 2 * VC : rl * VC;  // first element that the lane loads of a value row
+  const int v_at = v_first < D ? v_first * EB : 0;
+  const int v_second = v_first + 8 < D ? 16 : 0;  // second part of a value row, where it lies inside the row
 
   const int64_t krow = p.k_row_stride * EB, vrow = p.v_row_stride * EB;
-  auto place = [&](int key, const char* base, int64_t page_stride, int64_t row) {  // of one key (NARROW)
+  const int64_t kpage = p.k_page_stride * EB, vpage = p.v_page_stride * EB;
+  auto place = [&](int key, const char* base, int64_t page_stride, int64_t row) {  // of one key (kKeys)
     const int k = any_sees(key) ? key : seen.hi - 1;
     const int pg = page_of(a, k);
-    return base + checked(table[pg]) * page_stride * EB + (k - pg * p.page_size) * row;
+    return base + checked(table[pg]) * page_stride + (k - pg * p.page_size) * row;
   };
-  auto load_k = [&](int key0, int page) {
-    const int k = usable(key0 + kg * 8);
-    const char* at = kbase + checked(page) * p.k_page_stride * EB + (k - page_of(a, k) * p.page_size + (rl & 3)) * krow;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if constexpr (NARROW) at = place(key0 + kg * 8 + t * 4 + (rl & 3), kbase, p.k_page_stride, krow);
-#pragma unroll
-      for (int c = 0; c < KL; ++c) xk[t][c] = __builtin_nontemporal_load((const u32x4*)(at + k_at[c]));
-      if constexpr (!NARROW) at += 4 * krow;
+  // kHalves: the 16 keys from `key` on, or 16 of which one is seen (scalar)
+  const int half_mask = p.page_size - 1;
+  auto usable_half = [&](int key) {
+    const bool some = (key < seen.hi) & ((key + 16 > seen.lo) | (key < seen.sinks));
+    return some ? key : (seen.hi - 1) & ~15;
+  };
+  // page numbers of a tile.  kHalves: of its halves (scalar); kGroups: of the lane's groups for K (SWAP_K: two) and V
+  struct Pages {
+    int a, b, c;
+  };
+  typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+  // Tiles past the wave's last one are the range's last one again: loads are never skipped, so that the waits of the loop are
+  // for the loads they mean and not for all of them.
+  auto key_of = [&](int t) { return tile_key<kTile>(seen, t < t_end ? t : t_end - 1); };
+  auto pages_of = [&](int t) {
+    const int key0 = key_of(t);
+    if constexpr (PAGES == kHalves) {
+      const scalar_ptr entries = (scalar_ptr)(uintptr_t)table;
+      return Pages{entries[usable_half(key0) >> a.page_bits], entries[usable_half(key0 + 16) >> a.page_bits], 0};
+    } else if constexpr (PAGES == kGroups) {
+      return Pages{table[page_of(a, usable(key0 + kg * 8))], SWAP_K ? table[page_of(a, usable(key0 + (kg + 2) * 8))] : 0,
+                   table[page_of(a, usable(key0 + g * 8))]};
+    } else {
+      return Pages{0, 0, 0};
     }
   };
-  auto load_v = [&](int key0, int page, int vp) {
-    const int k = usable(key0 + g * 8);
-    const char* at = vbase + checked(page) * p.v_page_stride * EB + (k - page_of(a, k) * p.page_size) * vrow + v_at + vp * v_second;
+  auto half_at = [&](int key, int page, int64_t page_stride, int64_t row) {
+    const bool ok = (uint32_t)page < (uint32_t)a.p.num_pages;
+    bad_half |= !ok;
+    return (ok ? page : 0) * page_stride + (usable_half(key) & half_mask) * row;
+  };
+  // the lane's row in its half tile (kHalves) or in its group
+  const int64_t k_lane = ((PAGES == kHalves ? (kg & 1) * 8 : 0) + (rl & 3)) * krow;
+  const int v_bit = SWAP_V ? (rl >> 3) & 1 : 0;  // SWAP_V: which key of a pair the lane loads
+  const int64_t v_lane = ((PAGES == kHalves ? (g & 1) * 8 : 0) + v_bit) * vrow + v_at;
+  auto group_at = [&](int key, int page, int64_t page_stride, int64_t row) {
+    const int k = usable(key);
+    return checked(page) * page_stride + (k - page_of(a, k) * p.page_size) * row;
+  };
+  auto load_k = [&](u32x4 (&x)[2][KL], int key0, Pages pg) {
+    int64_t at[SWAP_K ? 2 : 1];                  // of the lane's row in half tile 0, for the loads of a pair
+    if constexpr (PAGES == kHalves) {
+      const int64_t h0 = half_at(key0, pg.a, kpage, krow), h1 = half_at(key0 + 16, pg.b, kpage, krow);
+      if constexpr (SWAP_K) at[0] = h0, at[1] = h1;
+      else at[0] = kg >= 2 ? h1 : h0;
+    } else if constexpr (PAGES == kGroups) {
+      at[0] = group_at(key0 + kg * 8, pg.a, kpage, krow);
+      if constexpr (SWAP_K) at[1] = group_at(key0 + (kg + 2) * 8, pg.b, kpage, krow);
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (NARROW) at = place(key0 + g * 8 + j, vbase, p.v_page_stride, vrow) + v_at + vp * v_second;
-      load_words(xv[j], at);
-      if constexpr (!NARROW) at += vrow;
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < (SWAP_K ? 2 : 1); ++i) {
+        const char* row;
+        if constexpr (PAGES == kKeys) row = place(key0 + (kg + 2 * i) * 8 + t * 4 + (rl & 3), kbase, kpage, krow);
+        else row = kbase + at[i] + (k_lane + t * 4 * krow);
+#pragma unroll
+        for (int c = i; c < KL; c += SWAP_K ? 2 : 1) x[t][c] = __builtin_nontemporal_load((const u32x4*)(row + k_at[c]));
+      }
+  };
+  auto load_v = [&](uint32_t (&x)[8][VWP], int key0, Pages pg, int vp) {
+    int64_t at = 0;
+    if constexpr (PAGES == kHalves) {
+      const int64_t h0 = half_at(key0, pg.a, vpage, vrow), h1 = half_at(key0 + 16, pg.b, vpage, vrow);
+      at = g >= 2 ? h1 : h0;
+    } else if constexpr (PAGES == kGroups) {
+      at = group_at(key0 + g * 8, pg.c, vpage, vrow);
+    }
+    const char* row = vbase + at + (v_lane + vp * v_second);
+#pragma unroll
+    for (int j = 0; j < 8; j += SWAP_V ? 2 : 1) {
+      if constexpr (PAGES == kKeys) row = place(key0 + g * 8 + j + v_bit, vbase, vpage, vrow) + v_at + vp * v_second;
+      constexpr int W = SWAP_V ? 2 * VWP : VWP;  // words of the load: two blocks of the row, or one
+      uint32_t w[W];
+      if constexpr (W == 2) *reinterpret_cast<u32x2*>(w) = __builtin_nontemporal_load((const u32x2*)row);
+      else *reinterpret_cast<u32x4*>(w) = __builtin_nontemporal_load((const u32x4*)row);
+#pragma unroll
+      for (int i = 0; i < W; ++i) x[j + i / VWP][i % VWP] = w[i];
+      row += (SWAP_V ? 2 : 1) * vrow;
     }
   };
 
-  // ---- the wave's tiles.  The keys of the next tile are requested as soon as the scores have taken those of this one, its
-  // values as soon as the output has: one tile in flight per wave and one set of registers for it; the page numbers of a
-  // tile are requested two tiles ahead. ---------------------------------------------------------------------------------
-  auto page_at = [&](int t, int group) -> int {
-    if constexpr (NARROW) return 0;
-    return table[page_of(a, usable(tile_key<kTile>(seen, t < t_end ? t : t_end - 1) + group * 8))];
-  };
-  int t = t_begin + wave;
-  int k_page = 0, v_page = 0, k_now = 0, v_now = 0;
-  if (t < t_end) {
-    const int kp = page_at(t, kg), vp = page_at(t, g);
-    k_page = page_at(t + 4, kg), v_page = page_at(t + 4, g);
-    if constexpr (!LATE) {
-      load_k(tile_key<kTile>(seen, t), kp);
-      load_v(tile_key<kTile>(seen, t), vp, 0);
-    }
-    k_now = kp, v_now = vp;
-  }
-  for (; t < t_end; t += 4) {
-    const int key0 = tile_key<kTile>(seen, t), key1 = tile_key<kTile>(seen, t + 4 < t_end ? t + 4 : t);
-    const bool more = t + 4 < t_end;
-    const int k_page2 = page_at(t + 8, kg), v_page2 = page_at(t + 8, g);
+  // ---- the wave's tiles, NB in flight.  As soon as the scores have taken the keys of a tile, those of the tile NB further
+  // on are requested into the same registers, and its values as soon as the output has taken them; the page numbers of a tile
+  // are requested another NB tiles ahead. ---------------------------------------------------------------------------------
+  Frag qf[NQ][KS];
+  Pages now = {0, 0};
+  auto body = [&](int t, u32x4 (&xk)[2][KL], uint32_t (&xv)[8][VWP], Pages& next) {
+    const int key0 = key_of(t);
+    const bool live = NB == 1 || t < t_end;
+    const int key1 = key_of(t + 4 * NB);
+    const Pages later = pages_of(t + 8 * NB);
     // a tile that every row sees in full needs no mask
-    bool full = true;
+    bool full = live;
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
-      full = full && key0 + kTile <= hi_r[n] && (key0 >= lo_r[n] || key0 + kTile <= seen.sinks);
+      full = full & (key0 + kTile <= hi_r[n]) & ((key0 >= lo_r[n]) | (key0 + kTile <= seen.sinks));
     full = __builtin_amdgcn_ballot_w64(full) == ~0ull;
-    if constexpr (LATE) load_k(key0, k_now);
+    if constexpr (LATE) load_k(xk, key0, now);
+    if constexpr (SWAP_K) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int c = 0; c < KL; c += 2)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t lo = xk[t][c][w], hi = xk[t][c + 1][w];
+            swap_half_rows(lo, hi);
+            xk[t][c][w] = lo, xk[t][c + 1][w] = hi;
+          }
+    }
     if (ragged) {
 #pragma unroll
       for (int c = 0; c < KL; ++c)
@@ -248,102 +303,151 @@ __global__ __launch_bounds__(256, 2) void attn_stream_kernel(CacheAttnArgs a) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) s[n][t] = Mma16<T>::mma(__builtin_bit_cast(Frag, w), qf[n][st], s[n][t]);
       }
-    if constexpr (!LATE)
-      if (more) load_k(key1, k_page);
+    if constexpr (!LATE) load_k(xk, key1, next);
     // ---- softmax: element e of half t is key key0 + g * 8 + t * 4 + e ---------------------------------------------------
-    Frag pf[NQ];
+    float z[NQ][8], top[NQ];
+    bool moves = false;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      float z[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = s[n][e >> 2][e & 3];
+      for (int e = 0; e < 8; ++e) z[n][e] = s[n][e >> 2][e & 3];
       if (capped) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = a.cap_out_log2 * tanhf(z[e] * cap_in);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] *= sc;
+        for (int e = 0; e < 8; ++e) z[n][e] = tanh_of(z[n][e] * inner);
       }
       if (!full) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int key = key0 + g * 8 + e;
-          const bool sees = key < hi_r[n] && (key >= lo_r[n] || key < seen.sinks);
-          z[e] = sees ? z[e] : -INFINITY;
+          const bool sees = live & (key < hi_r[n]) & ((key >= lo_r[n]) | (key < seen.sinks));
+          z[n][e] = sees ? z[n][e] : -INFINITY;
         }
       }
-      float top = z[0];
+      top[n] = z[n][0];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, z[e]);
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const bool moved = top > m_run[n] + 8.0f;
-      const float m_new = moved ? top : m_run[n];
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      T pr[8];
-      float sum = 0.f;
+      for (int e = 1; e < 8; ++e) top[n] = fmaxf(top[n], z[n][e]);
+      top[n] *= sc;
+      moves = moves | (top[n] > m_run[n] + 8.0f);
+    }
+    if (__builtin_amdgcn_ballot_w64(moves) != 0) {  // rare: only now do the four lanes of a row compare
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = __builtin_amdgcn_exp2f(z[e] - m_use);
-        sum += v;
-        pr[e] = (T)v;
-      }
-      pf[n] = *reinterpret_cast<Frag*>(pr);
-      if (__builtin_amdgcn_ballot_w64(moved) != 0) {
-        const float alpha = moved ? __builtin_amdgcn_exp2f(m_run[n] - m_use) : 1.0f;
+      for (int n = 0; n < NQ; ++n) {
+        float m = fmaxf(top[n], __shfl_xor(top[n], 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        m = m > m_run[n] + 8.0f ? m : m_run[n];
+        const float alpha = m == m_run[n] ? 1.0f : __builtin_amdgcn_exp2f(m_run[n] - m);
+        m_run[n] = m;
         l_run[n] *= alpha;
 #pragma unroll
         for (int j = 0; j < VC; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[n][j][e] *= alpha;
       }
+    }
+    Frag pf[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const float m_use = m_run[n] == -INFINITY ? 0.f : m_run[n];
+      T pr[8];
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = __builtin_amdgcn_exp2f(fmaf(z[n][e], sc, -m_use));
+        sum += v;
+        pr[e] = (T)v;
+      }
+      pf[n] = *reinterpret_cast<Frag*>(pr);
       l_run[n] += sum;                           // of the lane's own keys; the four lanes of a row meet at the end
-      m_run[n] = m_new;
     }
     // ---- output: words of 2 elements per key -> fragments of 8 keys per element -----------------------------------------
 #pragma unroll
     for (int vp = 0; vp < VP; ++vp) {
-      if constexpr (LATE) load_v(key0, v_now, vp);
+      if constexpr (LATE) load_v(xv, key0, now, vp);
+      if constexpr (SWAP_V) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+#pragma unroll
+          for (int w = 0; w < VWP; ++w) swap_half_rows(xv[j][w], xv[j + 1][w]);
+      }
       if (!full) {  // values of keys that no row sees: zero
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (!any_sees(key0 + g * 8 + j)) {
+          if (!(live & any_sees(key0 + g * 8 + j))) {
 #pragma unroll
             for (int w = 0; w < VWP; ++w) xv[j][w] = 0u;
           }
       }
+      auto product = [&](int j, u32x4 f) {       // element j of the lane's VC, keys g * 8 + 0..7
 #pragma unroll
-      for (int hp = 0; hp < VC / 2 / VP; ++hp) {
-        const int h = vp * (VC / 2 / VP) + hp;
-        uint32_t w[8];
+        for (int n = 0; n < NQ; ++n) acc[n][j] = Mma16<T>::mma(__builtin_bit_cast(Frag, f), pf[n], acc[n][j]);
+      };
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if constexpr (WIDE) w[j] = xv[j][hp];
-          else if (hp & 1) w[j] = Widen<T, FMT>::template two<true>(xv[j][hp >> 1]);
-          else w[j] = Widen<T, FMT>::template two<false>(xv[j][hp >> 1]);
-        }
-        u32x4 f0, f1;
+      for (int i = 0; i < VWP; ++i) {
+        if constexpr (WIDE) {                    // a word is two elements of a key
+          const int j = (vp * VWP + i) * 2;
+          u32x4 f0, f1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f0[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100);
-          f1[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302);
-        }
+          for (int k = 0; k < 4; ++k) {
+            f0[k] = __builtin_amdgcn_perm(xv[2 * k + 1][i], xv[2 * k][i], 0x05040100);
+            f1[k] = __builtin_amdgcn_perm(xv[2 * k + 1][i], xv[2 * k][i], 0x07060302);
+          }
+          product(j, f0);
+          product(j + 1, f1);
+        } else {                                 // four: bytes of two keys side by side first, widened as pairs of keys
+          u32x4 f0, f1, f2, f3;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          acc[n][2 * h] = Mma16<T>::mma(__builtin_bit_cast(Frag, f0), pf[n], acc[n][2 * h]);
-          acc[n][2 * h + 1] = Mma16<T>::mma(__builtin_bit_cast(Frag, f1), pf[n], acc[n][2 * h + 1]);
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t lo = __builtin_amdgcn_perm(xv[2 * k + 1][i], xv[2 * k][i], 0x05010400);
+            const uint32_t hi = __builtin_amdgcn_perm(xv[2 * k + 1][i], xv[2 * k][i], 0x07030602);
+            f0[k] = Widen<T, FMT>::template two<false>(lo);
+            f1[k] = Widen<T, FMT>::template two<true>(lo);
+            f2[k] = Widen<T, FMT>::template two<false>(hi);
+            f3[k] = Widen<T, FMT>::template two<true>(hi);
+          }
+          product(i * 4, f0);
+          product(i * 4 + 1, f1);
+          product(i * 4 + 2, f2);
+          product(i * 4 + 3, f3);
         }
       }
     }
-    if constexpr (!LATE)
-      if (more) load_v(key1, v_page, 0);
-    k_now = k_page, v_now = v_page;
-    k_page = k_page2, v_page = v_page2;
+    if constexpr (!LATE) load_v(xv, key1, next, 0);
+    now = next;
+    next = later;
+  };
+  const int t0 = t_begin + wave;
+  if (t0 < t_end) {
+    Pages ahead[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) ahead[u] = pages_of(t0 + 4 * u);
+    now = ahead[0];
+    if constexpr (!LATE) {
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        // (in the order of the loop: a wait counts what was requested later)
+        load_k(xk[u], key_of(t0 + 4 * u), ahead[u]);
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(xv[u], key_of(t0 + 4 * u), ahead[u], 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NB; ++u) ahead[u] = pages_of(t0 + 4 * (NB + u));
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        qf[n][s] = __builtin_bit_cast(Frag, (q_raw[n][s] & (q_inside(s) ? q_mask[n] : 0u)) ^ q_flip);
+    // (an odd tile out is computed with every key masked: with a way round it in the loop the compiler waits for all loads)
+    for (int t = t0; t < t_end; t += 4 * NB) {
+      body(t, xk[0], xv[0], ahead[0]);
+      if constexpr (NB == 2) body(t + 4, xk[1], xv[1], ahead[1]);
+    }
   }
-  const bool broken = __builtin_amdgcn_ballot_w64(bad) != 0;
+  const bool broken = __builtin_amdgcn_ballot_w64(bad || bad_half) != 0;
 
   // ---- merge of the four waves: 16 rows at a time -------------------------------------------------------------------------
-  const float v_scale = seq_scale(a.p.v_scale, a.p.v_scale_batch_stride, a.p.v_scale_head_stride, b, kvh);
+  const float v_scale = seq.v_scale;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int live = rows - (row0 + n * 16) < 16 ? rows - (row0 + n * 16) : 16;
@@ -360,9 +464,12 @@ __global__ __launch_bounds__(256, 2) void attn_stream_kernel(CacheAttnArgs a) {
         ml[(wave * 16 + rl) * 2 + 1] = l;
       }
 #pragma unroll
-      for (int e = 0; e < EH; ++e)                     // element (g * 4 + e0 + e) * VC + j of the row
+      for (int e = 0; e < EH; ++e) {                   // output row m = g * 4 + e0 + e is a block of VC elements
+        const int m = g * 4 + e;
+        const int block = SWAP_V ? (m & 7) * 2 + (m >> 3) : g * EH + e;
 #pragma unroll
-        for (int j = 0; j < VC; ++j) part[(wave * 16 + rl) * PITCH + (g * EH + e) * VC + j] = acc[n][j][e0 + e];
+        for (int j = 0; j < VC; ++j) part[(wave * 16 + rl) * PITCH + block * VC + j] = acc[n][j][e0 + e];
+      }
       __syncthreads();
       for (int i = tid; i < live * MD; i += 256) {
         const int r = i / MD, x = i - r * MD;
@@ -388,7 +495,7 @@ __global__ __launch_bounds__(256, 2) void attn_stream_kernel(CacheAttnArgs a) {
           if (d == 0 && p.lse != nullptr)
             p.lse[(int64_t)head * p.total_q + q_bos + tok] = empty ? INFINITY : m_use * 0.6931471805599453f + logf(sum);
         } else {
-          const int64_t at = (((int64_t)split * p.batch + b) * a.max_q + tok) * p.Hq + head;
+          const int64_t at = part_row(a, split, b, q_bos, tok) * p.Hq + head;
           a.part_o[at * DP + d] = o;
           if (d == 0) a.part_ml[at * 2] = m, a.part_ml[at * 2 + 1] = sum;
         }
@@ -397,61 +504,13 @@ __global__ __launch_bounds__(256, 2) void attn_stream_kernel(CacheAttnArgs a) {
   }
 }
 
-// Merges the key ranges: one thread per (sequence, token, head, element).
-template <typename T, int DP, int NQ>
-__global__ __launch_bounds__(256) void attn_stream_merge_kernel(CacheAttnArgs a) {
-  const FgFlashParams& p = a.p.base;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int d = (int)(i % DP);
-  const int64_t bth = i / DP;
-  const int head = (int)(bth % p.Hq);
-  const int tok = (int)(bth / p.Hq % a.max_q);
-  const int64_t b64 = bth / p.Hq / a.max_q;
-  if (b64 >= p.batch) return;
-  const int b = (int)b64;
-  const int q_bos = p.cu_seqlens_q[b];
-  const int q_len = p.cu_seqlens_q[b + 1] - q_bos;
-  if (q_len < a.min_q || q_len > a.max_q || tok >= q_len || d >= p.D) return;
-  if (q_bos < 0 || (int64_t)q_bos + q_len > p.total_q) return;
-  const int64_t reach = (int64_t)a.p.table_width * p.page_size;
-  const int k_said = p.seqused_k[b];
-  const int k_len = k_said < 0 ? 0 : (k_said < reach ? k_said : (int)reach);
-  // the ranges of the row's block that were written
-  const int row = tok * a.group + head % a.group;
-  const int row0 = row / (16 * NQ) * (16 * NQ), rows = q_len * a.group;
-  const int last_row = row0 + 16 * NQ < rows ? row0 + 16 * NQ - 1 : rows - 1;
-  const Seen seen = seen_by<kTile>(a, q_len, k_len, row0 / a.group, last_row / a.group);
-  const int per = range_tiles(a, seen.tiles);
-  int ns = per > 0 ? (seen.tiles + per - 1) / per : 1;
-  ns = ns < 1 ? 1 : (ns > a.splits ? a.splits : ns);
-  const int64_t step = (int64_t)p.batch * a.max_q * p.Hq, at = ((int64_t)b * a.max_q + tok) * p.Hq + head;
-  float m = -INFINITY;
-  for (int s = 0; s < ns; ++s) m = fmaxf(m, a.part_ml[(s * step + at) * 2]);
-  const float m_use = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o = 0.f;
-  for (int s = 0; s < ns; ++s) {
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[(s * step + at) * 2] - m_use);
-    l += a.part_ml[(s * step + at) * 2 + 1] * f;
-    o += a.part_o[(s * step + at) * DP + d] * f;
-  }
-  const bool empty = l == 0.f;
-  const float v_scale = seq_scale(a.p.v_scale, a.p.v_scale_batch_stride, a.p.v_scale_head_stride, b, head / a.group);
-  ((T*)p.out)[(int64_t)(q_bos + tok) * p.o_row_stride + (int64_t)head * p.o_head_stride + d] =
-      (T)(empty ? 0.f : o * (v_scale / l));
-  if (d == 0 && p.lse != nullptr)
-    p.lse[(int64_t)head * p.total_q + q_bos + tok] = empty ? INFINITY : m_use * 0.6931471805599453f + logf(l);
-}
-
-template <typename T, int FMT, int DP, int NQ, bool NARROW>
+template <typename T, int FMT, int DP, int NQ, int PAGES>
 int launch_stream(const CacheAttnArgs& a, hipStream_t st) {
   const FgFlashParams& p = a.p.base;
   const int64_t blocks = fg_cdiv((int64_t)a.max_q * a.group, 16 * NQ) * a.splits;
   FG_REQUIRE(blocks < ((int64_t)1 << 31), FG_ERR_UNSUPPORTED, "cache_attn_fwd: too many query rows for one launch");
-  hipLaunchKernelGGL((attn_stream_kernel<T, FMT, DP, NQ, NARROW>), dim3((unsigned)blocks, (unsigned)p.batch, (unsigned)p.Hk),
+  hipLaunchKernelGGL((attn_stream_kernel<T, FMT, DP, NQ, PAGES>), dim3((unsigned)blocks, (unsigned)p.batch, (unsigned)p.Hk),
                      dim3(256), 0, st, a);
-  if (a.splits > 1) {
-    const int64_t total = (int64_t)p.batch * a.max_q * p.Hq * DP;
-    hipLaunchKernelGGL((attn_stream_merge_kernel<T, DP, NQ>), dim3((unsigned)fg_cdiv(total, 256)), dim3(256), 0, st, a);
-  }
+  if (a.splits > 1) return launch_merge<T, DP, kTile, 16 * NQ, 4>(a, st);
   return fg_check_launch("cache_attn_fwd");
 }

@@ -20,10 +20,10 @@
 #pragma once
 
 constexpr int kTileKeys = 64;
-constexpr int kTileRows = 128;
 
 // POW2: the page size is a power of two.
-template <typename T, int FMT, int DP, bool POW2>
+// NQ: 16-row tiles of a wave; the workgroup's block has 64 * NQ rows.
+template <typename T, int FMT, int DP, bool POW2, int NQ>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
   typedef typename Mma16<T>::Frag Frag;
   constexpr bool WIDE = FMT == FG_CACHE_SAME;
@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
   constexpr int EPL = 16 / EB;                   // elements of a 16-byte load
   constexpr int KS = DP / 32;
   constexpr int DT = DP / 16;                    // output sub-tiles
-  constexpr int NQ = 2;
+  constexpr int ROWS = 64 * NQ;
   constexpr int RB = DP * 2;                     // bytes of a tile row
   constexpr int CPR = RB / 16;                   // 16-byte chunks of it: 16 or 8
   constexpr int TB = kTileKeys * RB;
@@ -45,32 +45,36 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rl = lane & 15, g = lane >> 4;
-  // Workgroup id -> (sequence, KV head), row block.  Workgroups go round-robin to the 8 XCDs; the row blocks of a pair all
-  // run on one, whose L2 then holds its keys.  The last rows of the sequences, which see the most, come first.
+  // Workgroup id -> (sequence, KV head), row block, key range.  Workgroups go round-robin to the 8 XCDs; what a pair has runs on
+  // one, whose L2 then holds its keys.  Unsplit: the last rows of the sequences, which see the most, come first.  Split: the
+  // row blocks that share a range run next to each other.
   const int pairs = p.batch * p.Hk;
   const int xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
   const int per_xcd = (pairs + 7) >> 3;
-  const int pair = xcd + 8 * (turn % per_xcd);
+  const int blocks = (a.max_q * a.group + ROWS - 1) / ROWS;
+  const int place = a.splits > 1 ? turn / blocks : turn;
+  const int pair = xcd + 8 * (place % per_xcd);
   if (pair >= pairs) return;
+  const int split = a.splits > 1 ? place / per_xcd : 0;
+  const int from_last = a.splits > 1 ? turn % blocks : place / per_xcd;
   const int b = pair / p.Hk, kvh = pair - b * p.Hk;
   const int G = a.group;
-  const int q_bos = p.cu_seqlens_q[b];
-  const int q_len = p.cu_seqlens_q[b + 1] - q_bos;
+  const Sequence seq = sequence(a, b, kvh);
+  const int q_bos = seq.q_bos, q_len = seq.q_len, k_len = seq.k_len;
   const int rows = q_len * G;
-  const int row0 = ((rows + kTileRows - 1) / kTileRows - 1 - turn / per_xcd) * kTileRows;
-  if (q_len < a.min_q || q_len > a.max_q || row0 < 0) return;
-  if (q_bos < 0 || (int64_t)q_bos + q_len > p.total_q) return;
-  const int64_t reach = (int64_t)a.p.table_width * p.page_size;
-  const int k_said = p.seqused_k[b];
-  const int k_len = k_said < 0 ? 0 : (k_said < reach ? k_said : (int)reach);
-  const int last_row = row0 + kTileRows < rows ? row0 + kTileRows - 1 : rows - 1;
+  const int row0 = ((rows + ROWS - 1) / ROWS - 1 - from_last) * ROWS;
+  if (!seq.mine || row0 < 0) return;
+  const int last_row = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
   const Seen seen = seen_by<kTileKeys>(a, q_len, k_len, row0 / G, last_row / G);
-  bool bad = k_said > reach;
+  bool bad = seq.too_long;
+  const int per = range_tiles<1>(a, seen.tiles);
+  const int t_begin = split * per;
+  const int t_end = t_begin + per < seen.tiles ? t_begin + per : seen.tiles;
+  if (split > 0 && t_begin >= t_end) return;     // range 0 always reports
 
   // t = sc * S with sc > 0, so that the largest t is sc times the largest S: the sign goes into the query (0: a query of 0)
-  const float k_scale = seq_scale(a.p.k_scale, a.p.k_scale_batch_stride, a.p.k_scale_head_stride, b, kvh);
   const bool capped = p.softcap > 0.f;
-  const float given = (capped ? a.cap_in : a.scale_log2) * k_scale;
+  const float given = (capped ? a.cap_in : a.scale_log2) * seq.k_scale;
   const uint32_t q_keep = given == 0.f ? 0u : ~0u, q_flip = given < 0.f ? 0x80008000u : 0u;
   const float inner = given == 0.f ? 1.0f : fabsf(given);
   const float sc = capped ? a.cap_out_log2 : inner;  // of S, or of tanh(inner * S)
@@ -79,17 +83,16 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
   const int D = p.D;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const int row = row0 + wave * 32 + n * 16 + rl;
+    const int row = row0 + wave * (16 * NQ) + n * 16 + rl;
     const bool ok = row < rows;
     const int tok = (ok ? row : row0) / G, head = kvh * G + (ok ? row : row0) % G;
     row_bounds(a, q_len, k_len, tok, lo_r[n], hi_r[n]);
     const T* q = (const T*)p.q + (int64_t)(q_bos + tok) * p.q_row_stride + (int64_t)head * p.q_head_stride;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      u32x4 v = {0u, 0u, 0u, 0u};
-      if (ok && s * 32 + g * 8 < D) v = *reinterpret_cast<const u32x4*>(q + s * 32 + g * 8);
-      v = (v & q_keep) ^ q_flip;
-      qf[n][s] = __builtin_bit_cast(Frag, v);
+      const int d = s * 32 + g * 8;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(q + (d < D ? d : 0));
+      qf[n][s] = __builtin_bit_cast(Frag, (v & (ok && d < D ? q_keep : 0u)) ^ q_flip);
     }
   }
   f32x4 acc[NQ][DT];
@@ -113,7 +116,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
   const bool alike = kpage == vpage && krow == vrow;
   u32x4 sk[NP], sv[NP];
   int page[NP];
-  auto any_sees = [&](int key) { return key < seen.hi && (key >= seen.lo || key < seen.sinks); };
+  auto any_sees = [&](int key) { return (key < seen.hi) & ((key >= seen.lo) | (key < seen.sinks)); };
   auto number = [&](int key) { return POW2 ? key >> a.page_bits : page_of(a, key); };
   auto slot_of = [&](int key) { return POW2 ? key & (p.page_size - 1) : key - page_of(a, key) * p.page_size; };
   // Pages of the thread's keys.  Where no row sees the key the entry of one that is seen is read: its page exists.
@@ -176,24 +179,24 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
   const int kr = (rl >> 2) * 8 + (rl & 3);       // key of the lane's MFMA row in half tile 0 of a 32-key part
   const int vk = g * 8 + (rl >> 2);              // key of the lane's address in a transposing read (and + 4)
 
-  if (seen.tiles > 0) {
-    look_up(0);
-    request(0);
-    if (seen.tiles > 1) look_up(1);
-    store(0, 0);
+  if (t_begin < t_end) {
+    look_up(t_begin);
+    request(t_begin);
+    if (t_begin + 1 < t_end) look_up(t_begin + 1);
+    store(t_begin, 0);
   }
   __syncthreads();
-  for (int t = 0; t < seen.tiles; ++t) {
-    const int buf = t & 1, key0 = tile_key<kTileKeys>(seen, t);
-    const bool more = t + 1 < seen.tiles;
+  for (int t = t_begin; t < t_end; ++t) {
+    const int buf = (t - t_begin) & 1, key0 = tile_key<kTileKeys>(seen, t);
+    const bool more = t + 1 < t_end;
     if (more) request(t + 1);
-    if (t + 2 < seen.tiles) look_up(t + 2);
+    if (t + 2 < t_end) look_up(t + 2);
     const char* const kt = lds[buf][0];
     const char* const vt = lds[buf][1];
     bool full = true;
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
-      full = full && key0 + kTileKeys <= hi_r[n] && (key0 >= lo_r[n] || key0 + kTileKeys <= seen.sinks);
+      full = full & (key0 + kTileKeys <= hi_r[n]) & ((key0 >= lo_r[n]) | (key0 + kTileKeys <= seen.sinks));
     full = __builtin_amdgcn_ballot_w64(full) == ~0ull;
     // ---- scores: s[n][u * 2 + t] element e is key u * 32 + g * 8 + t * 4 + e -----------------------------------------------
     f32x4 s[NQ][4];
@@ -218,7 +221,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
 #pragma unroll
         for (int h = 0; h < 4; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][h][e] = tanhf(s[n][h][e] * inner);
+          for (int e = 0; e < 4; ++e) s[n][h][e] = tanh_of(s[n][h][e] * inner);
       }
       if (!full) {
 #pragma unroll
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = key0 + (h >> 1) * 32 + g * 8 + (h & 1) * 4 + e;
-            const bool sees = key < hi_r[n] && (key >= lo_r[n] || key < seen.sinks);
+            const bool sees = (key < hi_r[n]) & ((key >= lo_r[n]) | (key < seen.sinks));
             s[n][h][e] = sees ? s[n][h][e] : -INFINITY;
           }
       }
@@ -236,7 +239,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) top[n] = fmaxf(top[n], s[n][h][e]);
       top[n] *= sc;
-      moves = moves || top[n] > m_run[n] + 8.0f;
+      moves = moves | (top[n] > m_run[n] + 8.0f);
     }
     if (__builtin_amdgcn_ballot_w64(moves) != 0) {
 #pragma unroll
@@ -290,16 +293,23 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
 
   // ---- epilogue: lane (row, g) holds elements 16 j + 4 g + e ---------------------------------------------------------------------
   const bool broken = __syncthreads_or(bad) != 0;
-  const float v_scale = seq_scale(a.p.v_scale, a.p.v_scale_batch_stride, a.p.v_scale_head_stride, b, kvh);
+  const float v_scale = seq.v_scale;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     float l = l_run[n];
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     if (broken) l = NAN;
-    const int row = row0 + wave * 32 + n * 16 + rl;
+    const int row = row0 + wave * (16 * NQ) + n * 16 + rl;
     if (row >= rows) continue;
     const int tok = row / G, head = kvh * G + row % G;
+    if (a.splits > 1) {
+      const int64_t at = part_row(a, split, b, q_bos, tok) * p.Hq + head;
+#pragma unroll
+      for (int j = 0; j < DT; ++j) *reinterpret_cast<f32x4*>(a.part_o + at * DP + j * 16 + g * 4) = acc[n][j];
+      if (g == 0) a.part_ml[at * 2] = m_run[n], a.part_ml[at * 2 + 1] = l;
+      continue;
+    }
     const bool empty = l == 0.f;
     const float f = empty ? 0.f : v_scale / l;
     T* const o = (T*)p.out + (int64_t)(q_bos + tok) * p.o_row_stride + (int64_t)head * p.o_head_stride;
@@ -316,14 +326,15 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
   }
 }
 
-template <typename T, int FMT, int DP>
+template <typename T, int FMT, int DP, int NQ>
 int launch_tile(const CacheAttnArgs& a, hipStream_t st) {
   const FgFlashParams& p = a.p.base;
-  const int64_t blocks = fg_cdiv((int64_t)a.max_q * a.group, kTileRows) * 8 * fg_cdiv((int64_t)p.batch * p.Hk, 8);
+  const int64_t blocks = fg_cdiv((int64_t)a.max_q * a.group, 64 * NQ) * a.splits * 8 * fg_cdiv((int64_t)p.batch * p.Hk, 8);
   FG_REQUIRE(blocks < ((int64_t)1 << 31), FG_ERR_UNSUPPORTED, "cache_attn_fwd: too many query rows for one launch");
   if (a.page_bits >= 0)
-    hipLaunchKernelGGL((attn_tile_kernel<T, FMT, DP, true>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_tile_kernel<T, FMT, DP, true, NQ>), dim3((unsigned)blocks), dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((attn_tile_kernel<T, FMT, DP, false>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_tile_kernel<T, FMT, DP, false, NQ>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+  if (a.splits > 1) return launch_merge<T, DP, kTileKeys, 64 * NQ, 1>(a, st);
   return fg_check_launch("cache_attn_fwd");
 }
