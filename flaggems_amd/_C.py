@@ -7,6 +7,7 @@ missing, or a call fails, the caller gets an exception.
 """
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -91,6 +92,10 @@ class FgCacheAttnParams(ctypes.Structure):
     ]
 
 
+# The same struct as one format, native sizes and alignment: packing it is several times faster than setting its fields.
+CACHE_ATTN_FORMAT = struct.Struct("@9P13q10i2fiPq2iqi2P4q")
+assert CACHE_ATTN_FORMAT.size == ctypes.sizeof(FgCacheAttnParams)
+
 _SIGNATURES = {
     "fg_last_error": (ctypes.c_char_p, []),
     "fg_abi_version": (c_int, []),
@@ -164,8 +169,8 @@ _SIGNATURES = {
     ),
     "fg_flash_attn_varlen_fwd": (c_int, [ctypes.POINTER(FgFlashParams), c_vp]),
     "fg_flash_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FgFlashParams), c_int]),
-    "fg_cache_attn_fwd": (c_int, [ctypes.POINTER(FgCacheAttnParams), c_vp]),
-    "fg_cache_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FgCacheAttnParams), c_int]),
+    "fg_cache_attn_fwd": (c_int, [c_vp, c_vp]),  # FgCacheAttnParams by reference, or packed bytes
+    "fg_cache_attn_workspace_bytes": (ctypes.c_size_t, [c_vp, c_int]),
 }
 
 _lib = None
@@ -242,11 +247,11 @@ def cache_format(cache_dtype, kv_cache_dtype="auto"):
     return fmt
 
 
-def head_scale(scale, heads, device, name):
+def head_scale(scale, heads, index, name):
     """(pointer, head stride) of an fp32 scale tensor: one number, or one for each head.  None: no scale (1)."""
     if scale is None:
         return None, 0
-    _check_scale(scale, device, name)
+    _check_scale(scale, index, name)
     if scale.numel() == 1:
         return scale.data_ptr(), 0
     if scale.shape != (heads,) or scale.stride(0) != 1:
@@ -255,11 +260,11 @@ def head_scale(scale, heads, device, name):
     return scale.data_ptr(), 1
 
 
-def sequence_scale(scale, batch, heads, device, name):
+def sequence_scale(scale, batch, heads, index, name):
     """(pointer, batch stride, head stride) of an fp32 scale tensor that expands to (batch, heads).  None: no scale (1)."""
     if scale is None:
-        return None, 0, 0
-    _check_scale(scale, device, name)
+        return 0, 0, 0
+    _check_scale(scale, index, name)
     if scale.numel() == 1:
         return scale.data_ptr(), 0, 0
     try:
@@ -269,11 +274,17 @@ def sequence_scale(scale, batch, heads, device, name):
     return full.data_ptr(), full.stride(0), full.stride(1)
 
 
-def _check_scale(scale, device, name):
+def _check_scale(scale, index, name):
     if not isinstance(scale, torch.Tensor):
         raise TypeError("%s must be a tensor, got %s" % (name, type(scale).__name__))
-    if scale.dtype != torch.float32 or scale.device != device:
-        raise ValueError("%s must be float32 on %s, got %s on %s" % (name, device, scale.dtype, scale.device))
+    if scale.dtype is not torch.float32 or scale.get_device() != index:
+        raise ValueError("%s must be float32 on the device of the other tensors (%d), got %s on %s" % (
+            name, index, scale.dtype, scale.device))
+
+
+def rows_dense(t, strides, inner):
+    """Whether t[i] is one dense block for every i; `inner`: the strides of its inner dimensions if it is (sizes of 1 aside)."""
+    return strides[1:] == inner or t.numel() == 0 or t[0].is_contiguous()
 
 
 def supported_dtype(dtype):

@@ -3,8 +3,8 @@
 //   write:  c = rn8(clamp(x / s[h], -max, max))     s fp32, one number or one for each KV head; c in e4m3 or e5m2
 //   read:   x = rn(c * s[h])                         one rounding, to fp16, bf16 or fp32 (16- and 32-bit caches: a copy)
 //
-// The quotient is the correctly rounded fp32 one before it is rounded to 8 bits, so a
-// value that lies half way between two 8-bit numbers goes to the even one.  Numbers beyond the format's largest are cut
+// The quotient is rounded to fp32 before it is rounded to 8 bits (see Quotient), so a value whose quotient is half way between
+// two 8-bit numbers goes to the even one.  Numbers beyond the format's largest are cut
 // to it, infinities too (the conversion instruction itself would turn them into NaN or infinity); NaN stays NaN.
 //
 // Both kernels are bound by HBM.
@@ -36,13 +36,34 @@ template <> struct Fp8<kE5M2> {
   }
 };
 
-// x / s, cut to the format's range.  The comparisons are false for NaN, which passes.
-template <int FMT> __device__ __forceinline__ float scaled(float x, float s) {
-  float q = x / s;
-  q = q > Fp8<FMT>::kMax ? Fp8<FMT>::kMax : q;
-  q = q < -Fp8<FMT>::kMax ? -Fp8<FMT>::kMax : q;
-  return q;
-}
+// x / s in fp32, cut to the format's range; NaN stays NaN.
+//   q = x * r,  r = 1 / s rounded to nearest;   q' = q + (x - q * s) * r
+// (the residual x - q * s is exact in one fused operation, so q' is x / s with a relative error of 2^-46 in front of its one
+// rounding: a quotient that is an fp32 number, such as a middle between two 8-bit ones, comes out as it is).  x is cut to
+// twice the range first, so that nothing overflows.  Seven plain operations an element instead of the eighteen of a division, which
+// alone would keep the vector ALU busy for 40 of the 76 us below.  Scales outside [2^-100, 2^100] are divided by.
+template <int FMT> struct Quotient {
+  float s, r, most;
+  bool plain;
+  __device__ __forceinline__ explicit Quotient(float scale) : s(scale), r(1.0f / scale) {
+    const float a = fabsf(scale);
+    plain = a >= 0x1p-100f && a <= 0x1p100f;     // false for NaN
+    most = 2.0f * Fp8<FMT>::kMax * a;
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    float q;
+    if (plain) {
+      const float c = __builtin_amdgcn_fmed3f(x, -most, most);
+      q = c * r;
+      q = fmaf(fmaf(-q, s, c), r, q);
+    } else {
+      q = x / s;
+      if (q != q) return q;
+    }
+    q = __builtin_amdgcn_fmed3f(q, -Fp8<FMT>::kMax, Fp8<FMT>::kMax);
+    return x != x ? x : q;
+  }
+};
 
 struct WriteArgs {
   const void* src[2];      // key, value rows
@@ -54,16 +75,20 @@ struct WriteArgs {
   const void* slots;
   int64_t num_tokens, num_slots;
   int row, D, block_size;  // row = H * D elements
+  int waves_log2;          // waves of a row: 1, 2 or 4
 };
 
-// One wave takes one (token, K or V) row, CH elements per lane and step: with CH = 16 two 16-byte loads (16-bit inputs)
-// become one 16-byte store.  A piece of CH elements lies in one head (CH divides D), so it has one scale.
+// One to four waves take a (token, K or V) row, CH elements per lane and piece: 16 bytes are loaded and 4 or 8 stored, both in
+// one stretch over a wave.  A piece lies in one head (CH divides D), so it has one scale.  Two pieces per lane are in flight.
+// [16384, 32, 128] K and V, bf16 to e4m3, random slots: 76 us = 5.3 TB/s (a large copy on this card: 5.0 to 5.4); one
+// wave per row with eight pieces in flight 86.
 template <typename T, int FMT, int CH, typename SLOT>
 __global__ __launch_bounds__(256) void cache_write8_kernel(WriteArgs a) {
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t tok = w >> 1;
+  const int64_t row = w >> a.waves_log2;
+  const int64_t tok = row >> 1;
   if (tok >= a.num_tokens) return;
-  const int which = (int)(w & 1);
+  const int which = (int)(row & 1);
   const int64_t slot = (int64_t)((const SLOT*)a.slots)[tok];
   if (slot < 0 || slot >= a.num_slots) return;  // a padding token; a slot outside the cache is dropped
   const int64_t blk = slot / a.block_size;
@@ -72,35 +97,49 @@ __global__ __launch_bounds__(256) void cache_write8_kernel(WriteArgs a) {
   char* dst = (which ? a.cache[1] : a.cache[0]) + blk * (which ? a.block_stride[1] : a.block_stride[0]) + off * a.row;
   const float* sc = which ? a.scale[1] : a.scale[0];
   const int64_t ss = which ? a.scale_stride[1] : a.scale_stride[0];
-  for (int i = (threadIdx.x & 63) * CH; i < a.row; i += 64 * CH) {
-    const float s = sc == nullptr ? 1.0f : sc[(i / a.D) * ss];
-    if constexpr (CH == 1) {
-      const float q = scaled<FMT>((float)src[i], s);
-      dst[i] = (char)(Fp8<FMT>::pack4(q, q, q, q) & 0xff);
-    } else {
-      constexpr int V = 16 / (int)sizeof(T) < CH ? 16 / (int)sizeof(T) : CH;
-      Pack<T, V> x[CH / V];
+  constexpr int U = 2;
+  const int step = (64 * CH) << a.waves_log2;
+  for (int i0 = (int)(w & ((1 << a.waves_log2) - 1)) * 64 * CH + (threadIdx.x & 63) * CH; i0 < a.row; i0 += step * U) {
+    Pack<T, CH> x[U];
+    float s[U];
 #pragma unroll
-      for (int j = 0; j < CH / V; ++j) x[j] = ld_pack_nt<T, V>(src + i + j * V);
-      uint32_t o[CH / 4];
-#pragma unroll
-      for (int j = 0; j < CH / 4; ++j) {
-        float q[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = scaled<FMT>((float)x[(j * 4 + e) / V].v[(j * 4 + e) % V], s);
-        o[j] = Fp8<FMT>::pack4(q[0], q[1], q[2], q[3]);
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * step;
+      if (i < a.row) {
+        x[u] = ld_pack_nt<T, CH>(src + i);
+        s[u] = sc == nullptr ? 1.0f : sc[(i / a.D) * ss];
       }
-      if constexpr (CH == 16)
-        __builtin_nontemporal_store(*reinterpret_cast<u32x4*>(o), reinterpret_cast<u32x4*>(dst + i));
-      else
-        __builtin_nontemporal_store(*reinterpret_cast<u32x2*>(o), reinterpret_cast<u32x2*>(dst + i));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * step;
+      if (i >= a.row) continue;
+      const Quotient<FMT> quotient(s[u]);
+      if constexpr (CH == 1) {
+        const float q = quotient((float)x[u].v[0]);
+        dst[i] = (char)(Fp8<FMT>::pack4(q, q, q, q) & 0xff);
+      } else {
+        uint32_t o[CH / 4];
+#pragma unroll
+        for (int j = 0; j < CH / 4; ++j) {
+          float q[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[e] = quotient((float)x[u].v[j * 4 + e]);
+          o[j] = Fp8<FMT>::pack4(q[0], q[1], q[2], q[3]);
+        }
+        if constexpr (CH == 8)
+          __builtin_nontemporal_store(*reinterpret_cast<u32x2*>(o), reinterpret_cast<u32x2*>(dst + i));
+        else
+          __builtin_nontemporal_store(o[0], reinterpret_cast<uint32_t*>(dst + i));
+      }
     }
   }
 }
 
 template <typename T, int FMT, int CH>
-int write_launch(const WriteArgs& a, int slot_is_i64, hipStream_t st) {
-  const unsigned grid = (unsigned)fg_cdiv(a.num_tokens * 2, 4);
+int write_launch(WriteArgs a, int slot_is_i64, hipStream_t st) {
+  a.waves_log2 = a.row > 256 * CH ? 2 : (a.row > 128 * CH ? 1 : 0);
+  const unsigned grid = (unsigned)fg_cdiv((a.num_tokens * 2) << a.waves_log2, 4);
   if (slot_is_i64) hipLaunchKernelGGL((cache_write8_kernel<T, FMT, CH, int64_t>), dim3(grid), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((cache_write8_kernel<T, FMT, CH, int32_t>), dim3(grid), dim3(256), 0, st, a);
   return fg_check_launch("reshape_and_cache_flash_8bit");
@@ -108,17 +147,11 @@ int write_launch(const WriteArgs& a, int slot_is_i64, hipStream_t st) {
 
 template <typename T, int FMT>
 int write_pieces(const WriteArgs& a, int slot_is_i64, hipStream_t st) {
-  auto fits = [&](int ch) {
-    const int64_t load = ch * (int64_t)sizeof(T) < 16 ? ch * (int64_t)sizeof(T) : 16;
-    for (int i = 0; i < 2; ++i)
-      if (!fg_aligned(a.src[i], load) || a.src_stride[i] * (int64_t)sizeof(T) % load != 0 || !fg_aligned(a.cache[i], ch) ||
-          a.block_stride[i] % ch != 0)
-        return false;
-    return a.D % ch == 0;
-  };
-  if (fits(16)) return write_launch<T, FMT, 16>(a, slot_is_i64, st);
-  if (fits(8)) return write_launch<T, FMT, 8>(a, slot_is_i64, st);
-  return write_launch<T, FMT, 1>(a, slot_is_i64, st);
+  constexpr int CH = 16 / (int)sizeof(T);
+  bool fits = a.D % CH == 0;
+  for (int i = 0; i < 2; ++i)
+    fits = fits && fg_aligned(a.src[i], 16) && a.src_stride[i] % CH == 0 && fg_aligned(a.cache[i], CH) && a.block_stride[i] % CH == 0;
+  return fits ? write_launch<T, FMT, CH>(a, slot_is_i64, st) : write_launch<T, FMT, 1>(a, slot_is_i64, st);
 }
 
 struct ReadArgs {
@@ -136,6 +169,16 @@ struct ReadArgs {
   int64_t num_rows, num_pages;
   int batch, row, D, page_size;
 };
+
+template <int PB> __device__ __forceinline__ Pack<char, PB> ld_bytes_nt(const char* p) {
+  if constexpr (PB >= 8) {
+    return ld_pack_nt<char, PB>(p);
+  } else {
+    Pack<char, PB> v;
+    __builtin_memcpy(&v, __builtin_assume_aligned(p, PB), PB);
+    return v;
+  }
+}
 
 // One wave takes one output row, K and V.  Its sequence is the last one that starts at or before the row: 64 starts are
 // compared at once.  Rows in front of the first and behind the last sequence are left alone; a page that the cache does
@@ -158,32 +201,56 @@ __global__ __launch_bounds__(256) void cache_read_kernel(ReadArgs a) {
   const int64_t page = pos >= 0 && page_at < a.table_width ? (int64_t)a.table[(int64_t)b * a.table_stride + page_at] : -1;
   const bool known = page >= 0 && page < a.num_pages;
   constexpr int IB = FMT == FG_CACHE_SAME ? (int)sizeof(U) : 1;  // bytes of a cached element
+  constexpr int PB = CH * IB;                                    // of a piece
+  const char* src[2];
+  U* dst[2];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const char* src = a.cache[which] + (known ? page * a.page_stride[which] + slot * (int64_t)a.row * IB : 0);
-    U* dst = (U*)a.out[which] + r * a.out_stride[which];
-    for (int i = lane * CH; i < a.row; i += 64 * CH) {
-      Pack<U, CH> o;
-      if constexpr (FMT == FG_CACHE_SAME) {
-        o = known ? ld_pack<U, CH>((const U*)src + i) : Pack<U, CH>{};
-      } else {
-        const float s = a.scale[which] == nullptr ? 1.0f : a.scale[which][(i / a.D) * a.scale_stride[which]];
-        if constexpr (CH == 1) {
-          const f32x2 x = Fp8<FMT>::template unpack2<false>((uint8_t)src[i]);
-          o.v[0] = (U)(known ? x[0] * s : 0.f);
-        } else {
-          const Pack<uint32_t, CH / 4> c = ld_pack<uint32_t, CH / 4>((const uint32_t*)(src + i));
+  for (int k = 0; k < 2; ++k) {
+    src[k] = a.cache[k] + (known ? page * a.page_stride[k] + slot * (int64_t)a.row * IB : 0);
+    dst[k] = (U*)a.out[k] + r * a.out_stride[k];
+  }
+  constexpr int N = 4;  // pieces of K and of V in flight
+  for (int i0 = lane * CH; i0 < a.row; i0 += 64 * CH * N) {
+    Pack<char, PB> c[N][2];
+    float s[N][2];
 #pragma unroll
-          for (int j = 0; j < CH / 4; ++j) {
-            const f32x2 lo = Fp8<FMT>::template unpack2<false>(c.v[j]), hi = Fp8<FMT>::template unpack2<true>(c.v[j]);
-            o.v[j * 4] = (U)(known ? lo[0] * s : 0.f);
-            o.v[j * 4 + 1] = (U)(known ? lo[1] * s : 0.f);
-            o.v[j * 4 + 2] = (U)(known ? hi[0] * s : 0.f);
-            o.v[j * 4 + 3] = (U)(known ? hi[1] * s : 0.f);
-          }
+    for (int n = 0; n < N; ++n) {
+      const int i = i0 + n * 64 * CH;
+      if (i < a.row) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          c[n][k] = ld_bytes_nt<PB>(src[k] + (int64_t)i * IB);
+          s[n][k] = FMT == FG_CACHE_SAME || a.scale[k] == nullptr ? 1.0f : a.scale[k][(i / a.D) * a.scale_stride[k]];
         }
       }
-      st_pack<U, CH>(dst + i, o);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = i0 + n * 64 * CH;
+      if (i >= a.row) continue;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        Pack<U, CH> o;
+        if constexpr (FMT == FG_CACHE_SAME) {
+          __builtin_memcpy(&o, &c[n][k], PB);
+          if (!known) o = Pack<U, CH>{};
+        } else if constexpr (CH == 1) {
+          const f32x2 x = Fp8<FMT>::template unpack2<false>((uint8_t)c[n][k].v[0]);
+          o.v[0] = (U)(known ? x[0] * s[n][k] : 0.f);
+        } else {
+          uint32_t w[CH / 4];
+          __builtin_memcpy(w, &c[n][k], PB);
+#pragma unroll
+          for (int j = 0; j < CH / 4; ++j) {
+            const f32x2 lo = Fp8<FMT>::template unpack2<false>(w[j]), hi = Fp8<FMT>::template unpack2<true>(w[j]);
+            o.v[j * 4] = (U)(known ? lo[0] * s[n][k] : 0.f);
+            o.v[j * 4 + 1] = (U)(known ? lo[1] * s[n][k] : 0.f);
+            o.v[j * 4 + 2] = (U)(known ? hi[0] * s[n][k] : 0.f);
+            o.v[j * 4 + 3] = (U)(known ? hi[1] * s[n][k] : 0.f);
+          }
+        }
+        st_pack_nt<U, CH>(dst[k] + i, o);
+      }
     }
   }
 }
@@ -194,7 +261,8 @@ int read_launch(const ReadArgs& a, hipStream_t st) {
   return fg_check_launch("gather_cache_flash");
 }
 
-// Pieces of 16 output bytes where everything is aligned for them, else single elements.
+// Pieces of 16 output bytes (one stretch over the wave: pieces of 32 take 125 us instead of 104 for 86 thousand rows of [8, 128])
+// where everything is aligned for them, else single elements.
 template <typename U, int FMT>
 int read_pieces(const ReadArgs& a, hipStream_t st) {
   constexpr int CH = 16 / (int)sizeof(U), IB = FMT == FG_CACHE_SAME ? (int)sizeof(U) : 1;
@@ -230,7 +298,7 @@ extern "C" int fg_reshape_and_cache_flash_8bit(const void* key, const void* valu
   if (num_tokens == 0 || (int64_t)H * D == 0 || num_blocks == 0) return FG_OK;
   FG_REQUIRE(key && value && key_cache && value_cache && slot_mapping, FG_ERR_INVALID,
              "reshape_and_cache_flash_8bit: null pointer");
-  FG_REQUIRE((int64_t)H * D < ((int64_t)1 << 30) && fg_cdiv(num_tokens * 2, 4) < ((int64_t)1 << 31), FG_ERR_UNSUPPORTED,
+  FG_REQUIRE((int64_t)H * D < ((int64_t)1 << 30) && num_tokens < ((int64_t)1 << 29), FG_ERR_UNSUPPORTED,
              "reshape_and_cache_flash_8bit: problem too large for one launch");
   FG_REQUIRE(key_block_stride >= (int64_t)block_size * H * D && value_block_stride >= (int64_t)block_size * H * D, FG_ERR_INVALID,
              "reshape_and_cache_flash_8bit: block stride smaller than a page (%d x %d x %d)", block_size, H, D);

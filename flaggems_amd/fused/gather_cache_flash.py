@@ -30,42 +30,57 @@ def gather_cache_flash(
     table, or not in the cache, gives zeros."""
     logger.debug("GEMS GATHER_CACHE_FLASH")
     num_blocks, block_size, num_heads, head_size = key_cache.shape
-    batch = cu_seqlens.numel() - 1
-    assert key_cache.dtype == value_cache.dtype and key_cache.shape == value_cache.shape, "the caches must match"
-    for t in (key_cache, value_cache):
-        assert t[0].is_contiguous() if num_blocks else True, "a page must be dense"
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.size(0) >= batch, "block_table must be int32 [batch, blocks]"
-    assert block_table.stride(1) == 1 or block_table.size(1) <= 1, "block_table must have contiguous rows"
-    assert cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.is_contiguous() and batch >= 0, "cu_seqlens must be contiguous int32 [batch + 1]"
+    batch = cu_seqlens.size(0) - 1
+    table_rows, table_width = block_table.shape
+    cache_dtype, index = key_cache.dtype, key_cache.get_device()
+    row_size = num_heads * head_size
+    page, row = (row_size, head_size, 1), (head_size, 1)
+    k_strides, v_strides, table_strides = key_cache.stride(), value_cache.stride(), block_table.stride()
+    assert value_cache.dtype is cache_dtype and value_cache.shape == key_cache.shape, "the caches must match"
+    assert _C.rows_dense(key_cache, k_strides, page) and _C.rows_dense(value_cache, v_strides, page), "a page must be dense"
+    assert block_table.dtype is torch.int32 and table_rows >= batch, "block_table must be int32 [batch, blocks]"
+    assert table_strides[1] == 1 or table_width <= 1, "block_table must have contiguous rows"
+    assert cu_seqlens.dtype is torch.int32 and batch >= 0 and cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous int32 [batch + 1]"
     if seq_starts is not None:
-        assert seq_starts.dtype == torch.int32 and seq_starts.is_contiguous() and seq_starts.shape == (batch,), "seq_starts must be contiguous int32 [batch]"
-    fmt = _C.cache_format(key_cache.dtype, kv_cache_dtype)
+        assert seq_starts.dtype is torch.int32 and seq_starts.is_contiguous() and seq_starts.shape == (batch,), "seq_starts must be contiguous int32 [batch]"
+    fmt = _C.cache_format(cache_dtype, kv_cache_dtype)
     if dtype is None:
-        dtype = key.dtype if key is not None else torch.bfloat16 if fmt is not None else key_cache.dtype
+        dtype = key.dtype if key is not None else torch.bfloat16 if fmt is not None else cache_dtype
     if fmt is None:
-        assert dtype == key_cache.dtype, "a cache of %s is read back as it is" % key_cache.dtype
+        assert dtype is cache_dtype, "a cache of %s is read back as it is" % cache_dtype
         fmt, k_scale, v_scale = _C.CACHE_SAME, None, None
     for t in (value_cache, block_table, cu_seqlens, seq_starts, key, value):
-        assert t is None or t.device == key_cache.device, "all tensors must be on one device"
-    k_ptr, k_stride = _C.head_scale(k_scale, num_heads, key_cache.device, "k_scale")
-    v_ptr, v_stride = _C.head_scale(v_scale, num_heads, key_cache.device, "v_scale")
+        assert t is None or t.get_device() == index, "all tensors must be on one device"
+    k_ptr, k_stride = _C.head_scale(k_scale, num_heads, index, "k_scale")
+    v_ptr, v_stride = _C.head_scale(v_scale, num_heads, index, "v_scale")
     dtype_id = _C.dtype_id(dtype)
-    with _C.device_guard(key_cache.device):
-        key, value = (torch.empty((num_rows, num_heads, head_size), dtype=dtype, device=key_cache.device) if t is None else t
-                      for t in (key, value))
-        for t in (key, value):
-            assert t.shape == (num_rows, num_heads, head_size) and t.dtype == dtype, "key/value must be [num_rows, heads, head_size] of %s" % dtype
-            assert t[0].is_contiguous() if num_rows else True, "a row must be dense"
-            assert num_rows <= 1 or t.stride(0) >= num_heads * head_size, "rows must not overlap"
-        if num_rows == 0 or batch == 0 or num_heads * head_size == 0:
+    device = key_cache.device
+    with _C.device_guard(device):
+        shape = (num_rows, num_heads, head_size)
+        if key is None:
+            key, key_row = torch.empty(shape, dtype=dtype, device=device), row_size
+        else:
+            key_row = _check_output(key, shape, row, dtype)
+        if value is None:
+            value, value_row = torch.empty(shape, dtype=dtype, device=device), row_size
+        else:
+            value_row = _check_output(value, shape, row, dtype)
+        if num_rows == 0 or batch == 0 or row_size == 0:
             return key, value
         rc = _C.lib().fg_gather_cache_flash(
             key_cache.data_ptr(), value_cache.data_ptr(), key.data_ptr(), value.data_ptr(), block_table.data_ptr(),
-            block_table.stride(0), block_table.size(1), cu_seqlens.data_ptr(),
-            seq_starts.data_ptr() if seq_starts is not None else None, batch, num_rows, num_heads, head_size, block_size,
-            num_blocks, key_cache.stride(0), value_cache.stride(0),
-            max(key.stride(0), num_heads * head_size), max(value.stride(0), num_heads * head_size),
-            k_ptr, k_stride, v_ptr, v_stride, dtype_id, fmt, _C.current_stream(key_cache.device),
+            table_strides[0], table_width, cu_seqlens.data_ptr(), None if seq_starts is None else seq_starts.data_ptr(),
+            batch, num_rows, num_heads, head_size, block_size, num_blocks, k_strides[0], v_strides[0], key_row, value_row,
+            k_ptr, k_stride, v_ptr, v_stride, dtype_id, fmt, _C.current_stream(device),
         )
-    _C.check(rc, "fg_gather_cache_flash")
+    if rc:
+        _C.check(rc, "fg_gather_cache_flash")
     return key, value
+
+
+def _check_output(given, shape, row, dtype):
+    """The elements between rows of an output that the caller gave."""
+    assert given.shape == shape and given.dtype is dtype, "key/value must be [num_rows, heads, head_size] of %s" % dtype
+    assert _C.rows_dense(given, given.stride(), row), "a row must be dense"
+    assert shape[0] <= 1 or given.stride(0) >= shape[1] * shape[2], "rows must not overlap"
+    return max(given.stride(0), shape[1] * shape[2])

@@ -141,68 +141,80 @@ def mha_varlan_fwd(
     return out, q, k, v, lse, philox_args, unused, probs
 
 
+# Scratch sizes by everything they depend on: sizes, masks and the device (one library call less for a shape seen before).
+_cache_attn_scratch = {}
+
+
 def cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, page_table, alibi_slopes, max_seqlen_q, max_seqlen_k,
                    softmax_scale, is_causal, window_size_left, window_size_right, softcap, num_sink_tokens, k_descale,
-                   v_descale):
-    """Attention over an 8-bit paged cache, or under a window with sink tokens: validation + launch.  Returns (out, lse)."""
+                   v_descale, return_lse=True):
+    """Attention over an 8-bit paged cache, or under a window with sink tokens: validation + launch.  Returns (out, lse);
+    lse is None where it is not asked for."""
     assert q.is_cuda and k.is_cuda and v.is_cuda
-    assert q.dtype in (torch.float16, torch.bfloat16), "FlashAttention only support fp16 and bf16 data type"
-    assert k.dtype == v.dtype
-    fmt = _C.cache_format(k.dtype)
-    assert fmt is not None or k.dtype == q.dtype, "the cache must hold q's type or 8-bit floats"
+    dtype, cache_dtype, index = q.dtype, k.dtype, q.get_device()
+    assert dtype is torch.bfloat16 or dtype is torch.float16, "FlashAttention only support fp16 and bf16 data type"
+    assert v.dtype is cache_dtype
+    fmt = _C.cache_format(cache_dtype)
+    assert fmt is not None or cache_dtype is dtype, "the cache must hold q's type or 8-bit floats"
     total_q, num_heads, head_size = q.shape
-    num_pages, block_size, num_heads_k, _ = k.shape
-    batch = cu_seqlens_q.numel() - 1
-    assert k.shape == v.shape == (num_pages, block_size, num_heads_k, head_size)
-    for t in (q, k, v):
-        assert t.stride(-1) == 1, "Input tensor must have contiguous last dimension"
-    assert page_table is not None and page_table.dtype == torch.int32 and page_table.dim() == 2
-    assert page_table.stride(-1) == 1 or page_table.size(1) <= 1
-    assert page_table.size(0) >= batch and page_table.size(1) > 0
-    assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.dim() == 1
+    num_pages, block_size, num_heads_k, cache_size = k.shape
+    batch = cu_seqlens_q.size(0) - 1
+    assert v.shape == k.shape and cache_size == head_size
+    q_row, q_head, q_unit = q.stride()
+    k_page, k_row, k_head, k_unit = k.stride()
+    v_page, v_row, v_head, v_unit = v.stride()
+    assert q_unit == k_unit == v_unit == 1, "Input tensor must have contiguous last dimension"
+    assert page_table is not None and page_table.dtype is torch.int32 and page_table.dim() == 2
+    table_rows, table_width = page_table.shape
+    table_stride, table_unit = page_table.stride()
+    assert table_rows >= batch and table_width > 0 and (table_unit == 1 or table_width == 1)
+    assert cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.is_contiguous()
     assert seqused_k is not None, "the paged kernel takes key lengths from seqused_k"
-    assert seqused_k.dtype == torch.int32 and seqused_k.is_contiguous() and seqused_k.shape == (batch,)
+    assert seqused_k.dtype is torch.int32 and seqused_k.is_contiguous() and seqused_k.shape == (batch,)
     assert num_heads % num_heads_k == 0, "Number of heads in key/value must divide number of heads in query"
     assert num_sink_tokens >= 0, "num_sink_tokens must not be negative"
-    for t in (k, v, page_table, cu_seqlens_q, seqused_k, out):
-        assert t is None or t.device == q.device, "all tensors must be on one device"
+    assert k.get_device() == v.get_device() == page_table.get_device() == cu_seqlens_q.get_device() == seqused_k.get_device() == index and (
+        out is None or out.get_device() == index), "all tensors must be on one device"
     if alibi_slopes is not None:
         raise NotImplementedError("alibi_slopes are not supported with an 8-bit cache or sink tokens")
     if out is not None:
-        assert out.stride(-1) == 1 and out.dtype == q.dtype and out.shape == (total_q, num_heads, head_size)
-    with _C.device_guard(q.device):
+        o_row, o_head, o_unit = out.stride()
+        assert o_unit == 1 and out.dtype is dtype and out.shape == (total_q, num_heads, head_size)
+    else:
+        o_row, o_head = num_heads * head_size, head_size
+    if fmt is None:
+        fmt, k_scale, v_scale = _C.CACHE_SAME, (0, 0, 0), (0, 0, 0)
+    else:
+        k_scale = _C.sequence_scale(k_descale, batch, num_heads_k, index, "k_descale")
+        v_scale = _C.sequence_scale(v_descale, batch, num_heads_k, index, "v_descale")
+    device = q.device
+    with _C.device_guard(device):
         if out is None:
-            out = torch.empty((total_q, num_heads, head_size), dtype=q.dtype, device=q.device)
-        lse = torch.empty((num_heads, total_q), dtype=torch.float, device=q.device)
-        if total_q > 0 and batch > 0:
-            c = _C.FgCacheAttnParams()
-            p = c.base
-            p.q, p.k_cache, p.v_cache, p.out, p.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
-            p.cu_seqlens_q, p.seqused_k, p.block_table = cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), page_table.data_ptr()
-            p.q_row_stride, p.q_head_stride, _ = q.stride()
-            p.o_row_stride, p.o_head_stride, _ = out.stride()
-            p.k_page_stride, p.k_row_stride, p.k_head_stride, _ = k.stride()
-            p.v_page_stride, p.v_row_stride, p.v_head_stride, _ = v.stride()
-            p.block_table_stride = page_table.stride(0)
-            p.total_q = total_q
-            p.batch, p.Hq, p.Hk, p.D, p.page_size = batch, num_heads, num_heads_k, head_size, block_size
-            p.max_seqlen_q, p.max_seqlen_k = int(max_seqlen_q), int(max_seqlen_k)
-            p.is_causal = 1 if is_causal else 0
-            p.window_left, p.window_right = int(window_size_left), int(window_size_right)
-            p.softmax_scale, p.softcap = float(softmax_scale), float(softcap)
-            p.dtype = _C.dtype_id(q.dtype)
-            c.cache_format = _C.CACHE_SAME if fmt is None else fmt
-            c.num_sink_tokens, c.num_pages, c.table_width = int(num_sink_tokens), num_pages, page_table.size(1)
-            if fmt is not None:
-                c.k_scale, c.k_scale_batch_stride, c.k_scale_head_stride = _C.sequence_scale(
-                    k_descale, batch, num_heads_k, q.device, "k_descale")
-                c.v_scale, c.v_scale_batch_stride, c.v_scale_head_stride = _C.sequence_scale(
-                    v_descale, batch, num_heads_k, q.device, "v_descale")
-            ws_bytes = _C.lib().fg_cache_attn_workspace_bytes(ctypes.byref(c), q.device.index or 0)
-            if ws_bytes > 0:
-                ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-                p.workspace, p.workspace_bytes = ws.data_ptr(), ws_bytes
-            rc = _C.lib().fg_cache_attn_fwd(ctypes.byref(c), _C.current_stream(q.device))
+            out = torch.empty((total_q, num_heads, head_size), dtype=dtype, device=device)
+        lse = torch.empty((num_heads, total_q), dtype=torch.float, device=device) if return_lse else None
+        if total_q == 0 or batch == 0:
+            return out, lse
+        sizes = (batch, num_heads, num_heads_k, head_size, block_size, int(max_seqlen_q), int(max_seqlen_k), 1 if is_causal else 0,
+                 int(window_size_left), int(window_size_right))
+
+        def packed(ws, ws_bytes):
+            return _C.CACHE_ATTN_FORMAT.pack(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), page_table.data_ptr(), 0,
+                q_row, q_head, o_row, o_head, k_page, k_row, k_head, v_page, v_row, v_head, table_stride, 0, total_q,
+                *sizes, softmax_scale, softcap, _C.dtype_id(dtype), ws, ws_bytes, fmt, num_sink_tokens, num_pages, table_width,
+                k_scale[0], v_scale[0], k_scale[1], k_scale[2], v_scale[1], v_scale[2])
+
+        key = (sizes, total_q, num_sink_tokens, fmt, index)
+        ws_bytes = _cache_attn_scratch.get(key)
+        if ws_bytes is None:
+            ws_bytes = _C.lib().fg_cache_attn_workspace_bytes(packed(0, 0), index)
+            if len(_cache_attn_scratch) >= 4096:
+                _cache_attn_scratch.clear()
+            _cache_attn_scratch[key] = ws_bytes
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes > 0 else None
+        rc = _C.lib().fg_cache_attn_fwd(packed(0 if ws is None else ws.data_ptr(), ws_bytes), _C.current_stream(device))
+        if rc:
             _C.check(rc, "fg_cache_attn_fwd")
     return out, lse
 
@@ -282,7 +294,7 @@ def flash_attn_varlen_func(
             raise NotImplementedError("q_descale: the query is not quantized on this path")
         out, softmax_lse = cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, block_table, alibi_slopes, max_seqlen_q,
                                           max_seqlen_k, softmax_scale, causal, left, right, softcap, num_sink_tokens,
-                                          k_descale, v_descale)
+                                          k_descale, v_descale, return_softmax_lse)
         return (out, softmax_lse) if return_softmax_lse else out
     assert num_sink_tokens >= 0, "num_sink_tokens must not be negative"
     out, q, k, v, softmax_lse, *_ = mha_varlan_fwd(

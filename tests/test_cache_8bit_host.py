@@ -41,8 +41,8 @@ class Calls(Harness):
         self.inside("k_scale", ksc, 4, [(H, kss)])
         self.inside("v_scale", vsc, 4, [(H, vss)])
 
-    def chk_fg_cache_attn_fwd(self, ref, stream):
-        c = ref._obj
+    def chk_fg_cache_attn_fwd(self, packed, stream):
+        c = _C.FgCacheAttnParams.from_buffer_copy(packed)
         p = c.base
         e = 2 if c.cache_format == _C.CACHE_SAME else 1
         self.inside("q", p.q, 2, [(p.total_q, p.q_row_stride), (p.Hq, p.q_head_stride), (p.D, 1)])
@@ -183,7 +183,7 @@ def test_attention_hands_over_what_it_was_given(calls):
         attend(kc, vc, k_descale=s, v_descale=s)
     attend(kc.float().bfloat16(), vc.float().bfloat16(), window_size=(9, 0), num_sink_tokens=4, q_descale=1, k_descale="ignored")
     assert calls.check_all() == ["fg_cache_attn_fwd"] * 7
-    last = [a for n, a in calls.rec.calls if n == "fg_cache_attn_fwd"][-1][0]._obj
+    last = _C.FgCacheAttnParams.from_buffer_copy([a for n, a in calls.rec.calls if n == "fg_cache_attn_fwd"][-1][0])
     assert (last.cache_format, last.num_sink_tokens, last.base.window_left, last.table_width, last.num_pages) == (_C.CACHE_SAME, 4, 9, 3, 6)
     assert last.k_scale is None
     before = len(calls.rec.calls)

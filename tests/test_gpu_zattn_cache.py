@@ -1,4 +1,5 @@
 """GPU parity of attention over an 8-bit paged cache and of sliding windows with sink tokens, against the 64-bit oracle."""
+import importlib
 import random
 
 import pytest
@@ -157,6 +158,7 @@ def test_without_a_workspace(gpu, monkeypatch):
 
     real = _C.lib()
     monkeypatch.setattr(_C, "lib", lambda: Stingy())
+    monkeypatch.setattr(importlib.import_module("flaggems_amd.ops.attention"), "_cache_attn_scratch", {})
     run_and_check(gpu, [(1, 9000), (1, 37)], 8, 2, 128, 16, torch.bfloat16, "e4m3")
 
 
