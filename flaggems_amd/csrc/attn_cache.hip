@@ -98,20 +98,22 @@ Plan make_plan(const FgCacheAttnParams& c) {
   const int G = p.Hq / p.Hk;
   const int64_t cus = num_cu();
   Plan plan = {};
-  const int few = 32 / G > 1 ? 32 / G : 1;
-  plan.tile = p.D <= 128 && p.max_seqlen_q > few;
-  plan.stream_q = plan.tile ? few : p.max_seqlen_q;
-  // every sequence as long as the longest: the stream kernel has none to take
-  if (plan.tile && (int64_t)p.total_q >= (int64_t)p.batch * p.max_seqlen_q) plan.stream_q = 0;
-  const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
-  plan.pages = pow2 && p.page_size >= 16 ? kHalves : (p.page_size % 8 == 0 ? kGroups : kKeys);
-  plan.nq = plan.pages != kKeys && p.D <= 128 && (int64_t)plan.stream_q * G > 16 ? 2 : 1;
   // the most keys that one row block of `q` tokens may see
   auto keys_of = [&](int64_t q, int tile) {
     int64_t keys = p.max_seqlen_k > 0 ? p.max_seqlen_k : 1;
     const int64_t window = (int64_t)p.window_left + q + c.num_sink_tokens + 2 * tile;
     return p.window_left >= 0 && window < keys ? window : keys;
   };
+  const int few = 32 / G > 1 ? 32 / G : 1;
+  plan.tile = p.D <= 128 && p.max_seqlen_q > few;
+  plan.stream_q = plan.tile ? few : p.max_seqlen_q;
+  // The tile kernel takes the short sequences too where all are as long as the longest, so that there are none, and where no row
+  // sees more than 1024 keys: a launch of its own costs more than such a sequence does here.
+  const bool even = (int64_t)p.total_q >= (int64_t)p.batch * p.max_seqlen_q;
+  if (plan.tile && (even || keys_of(fg_cdiv(64, G), kTileKeys) <= 1024)) plan.stream_q = 0;
+  const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
+  plan.pages = pow2 && p.page_size >= 16 ? kHalves : (p.page_size % 8 == 0 ? kGroups : kKeys);
+  plan.nq = plan.pages != kKeys && p.D <= 128 && (int64_t)plan.stream_q * G > 16 ? 2 : 1;
   const size_t row = (size_t)p.Hq * (padded_dim(p.D) + 2) * sizeof(float);
   plan.splits = 1;
   if (plan.stream_q > 0) {
@@ -131,7 +133,6 @@ Plan make_plan(const FgCacheAttnParams& c) {
     if (plan.splits > 1) plan.stream_bytes = (plan.splits * row * p.batch * plan.stream_q + 15) / 16 * 16;
   }
   if (plan.tile) {
-    const bool even = plan.stream_q == 0;
     const int dp = padded_dim(p.D);
     double best = 0;
     for (int nq = 1; nq <= 2; ++nq) {

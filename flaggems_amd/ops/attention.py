@@ -143,6 +143,7 @@ def mha_varlan_fwd(
 
 # Scratch sizes by everything they depend on: sizes, masks and the device (one library call less for a shape seen before).
 _cache_attn_scratch = {}
+_INT32_MAX = 2 ** 31 - 1
 
 
 def cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, page_table, alibi_slopes, max_seqlen_q, max_seqlen_k,
@@ -194,8 +195,9 @@ def cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, page_table, alibi_slop
         lse = torch.empty((num_heads, total_q), dtype=torch.float, device=device) if return_lse else None
         if total_q == 0 or batch == 0:
             return out, lse
-        sizes = (batch, num_heads, num_heads_k, head_size, block_size, int(max_seqlen_q), int(max_seqlen_k), 1 if is_causal else 0,
-                 int(window_size_left), int(window_size_right))
+        sizes = (batch, num_heads, num_heads_k, head_size, block_size, min(max_seqlen_q, _INT32_MAX), min(max_seqlen_k, _INT32_MAX),
+                 1 if is_causal else 0, min(max(window_size_left, -1), _INT32_MAX), min(max(window_size_right, -1), _INT32_MAX))
+        num_sink_tokens = min(num_sink_tokens, _INT32_MAX)
 
         def packed(ws, ws_bytes):
             return _C.CACHE_ATTN_FORMAT.pack(

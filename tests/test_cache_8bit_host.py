@@ -350,3 +350,13 @@ def test_oracle_attention_against_scalar_sums():
             assert max(abs(float(r["out"][row, h, i]) - num[i] / den) for i in range(8)) < 1e-9
     r = O.cache_attention(q, kc, vc, cu, torch.tensor([1, 0], dtype=torch.int32), table, 0.3)
     assert torch.isinf(r["lse"][:, [0, 1, 3]]).all() and (r["out"][[0, 1, 3]] == 0).all() and torch.isfinite(r["lse"][:, 2]).all()
+
+
+def test_bounds_beyond_32_bits_are_cut(calls):
+    """A window, a number of sinks or a length limit of any size is passed on as the largest that the parameters hold."""
+    kc, vc = cache()
+    attend(kc, vc, window_size=(1 << 40, 1 << 50), num_sink_tokens=1 << 33)
+    attend(kc, vc, window_size=(-7, -5))
+    a, b = (_C.FgCacheAttnParams.from_buffer_copy(c[0]) for n, c in calls.rec.calls if n == "fg_cache_attn_fwd")
+    assert (a.base.window_left, a.base.window_right, a.num_sink_tokens) == (2 ** 31 - 1,) * 3
+    assert (b.base.window_left, b.base.window_right, b.num_sink_tokens) == (-1, -1, 0)
