@@ -2,6 +2,8 @@
 // Included by attn_cache.hip inside its unnamed namespace, in front of attn_stream.h and attn_tile.h.
 #pragma once
 
+constexpr int64_t kMostBlocks = (int64_t)1 << 24;  // of 256 threads: a launch counts threads in 32 bits
+
 struct CacheAttnArgs {
   FgCacheAttnParams p;
   float scale_log2;            // softmax_scale * log2(e)             (softcap == 0)
@@ -258,6 +260,7 @@ template <typename T, int DP, int TILE, int ROWS, int UNIT>
 int launch_merge(const CacheAttnArgs& a, hipStream_t st) {
   const FgFlashParams& p = a.p.base;
   const int64_t rows = (int64_t)a.max_q * p.Hq;
+  FG_REQUIRE(rows < kMostBlocks, FG_ERR_UNSUPPORTED, "cache_attn_fwd: too many query rows for one launch");
   if (a.splits > 8)
     hipLaunchKernelGGL((attn_merge_kernel<T, DP, TILE, ROWS, UNIT, true>), dim3((unsigned)rows, (unsigned)p.batch), dim3(256), 0, st, a);
   else

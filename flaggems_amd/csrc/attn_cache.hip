@@ -178,7 +178,17 @@ int check_params(const FgCacheAttnParams* c) {
                  al(p.v_cache, n, p.v_row_stride, p.v_head_stride, p.v_page_stride),
              FG_ERR_UNSUPPORTED, "cache_attn_fwd: q/k/v rows must be 16-byte aligned");
   FG_REQUIRE(p.batch < 65536 && p.Hk < 65536, FG_ERR_UNSUPPORTED, "cache_attn_fwd: batch/heads exceed the grid");
+  // (key numbers, a tile or a few past the last one too, are 32-bit integers in the kernels)
+  FG_REQUIRE((int64_t)c->table_width * p.page_size <= INT_MAX - 65536, FG_ERR_UNSUPPORTED,
+             "cache_attn_fwd: a row of the block table spans %lld keys", (long long)c->table_width * p.page_size);
   return FG_OK;
+}
+
+// The call with its longest sequence no longer than all tokens together: the grids and the scratch go by it.
+FgCacheAttnParams bounded(const FgCacheAttnParams& given) {
+  FgCacheAttnParams c = given;
+  c.base.max_seqlen_q = (int)std::min((int64_t)c.base.max_seqlen_q, (int64_t)c.base.total_q);
+  return c;
 }
 
 }  // namespace
@@ -186,17 +196,17 @@ int check_params(const FgCacheAttnParams* c) {
 extern "C" size_t fg_cache_attn_workspace_bytes(const FgCacheAttnParams* c, int device) {
   (void)device;
   if (c == nullptr || c->base.batch <= 0 || c->base.total_q <= 0 || check_params(c) != FG_OK) return 0;
-  const Plan plan = make_plan(*c);
+  const Plan plan = make_plan(bounded(*c));
   return plan.stream_bytes + plan.tile_bytes;
 }
 
 extern "C" int fg_cache_attn_fwd(const FgCacheAttnParams* c, void* stream) {
   const int rc = check_params(c);
   if (rc != FG_OK) return rc;
-  const FgFlashParams& p = c->base;
-  if (p.batch == 0 || p.total_q == 0) return FG_OK;
+  if (c->base.batch == 0 || c->base.total_q == 0) return FG_OK;
   CacheAttnArgs a;
-  a.p = *c;
+  a.p = bounded(*c);
+  const FgFlashParams& p = a.p.base;
   if (c->cache_format == FG_CACHE_SAME) a.p.k_scale = a.p.v_scale = nullptr;
   const float log2e = 1.4426950408889634f;
   a.scale_log2 = p.softmax_scale * log2e;
@@ -210,7 +220,7 @@ extern "C" int fg_cache_attn_fwd(const FgCacheAttnParams* c, void* stream) {
   a.page_magic = (uint32_t)(((uint64_t)1 << (31 + s)) / (uint64_t)p.page_size + 1);
   a.page_shift = 31 + s;
   a.page_bits = ((int64_t)1 << s) == p.page_size ? s : -1;
-  const Plan plan = make_plan(*c);
+  const Plan plan = make_plan(a.p);
   const bool scratch = p.workspace != nullptr && fg_aligned(p.workspace, 16) && (size_t)p.workspace_bytes >= plan.stream_bytes + plan.tile_bytes;
   const int dp = padded_dim(p.D);
   hipStream_t st = (hipStream_t)stream;

@@ -508,7 +508,7 @@ template <typename T, int FMT, int DP, int NQ, int PAGES>
 int launch_stream(const CacheAttnArgs& a, hipStream_t st) {
   const FgFlashParams& p = a.p.base;
   const int64_t blocks = fg_cdiv((int64_t)a.max_q * a.group, 16 * NQ) * a.splits;
-  FG_REQUIRE(blocks < ((int64_t)1 << 31), FG_ERR_UNSUPPORTED, "cache_attn_fwd: too many query rows for one launch");
+  FG_REQUIRE(blocks < kMostBlocks, FG_ERR_UNSUPPORTED, "cache_attn_fwd: too many query rows for one launch");
   hipLaunchKernelGGL((attn_stream_kernel<T, FMT, DP, NQ, PAGES>), dim3((unsigned)blocks, (unsigned)p.batch, (unsigned)p.Hk),
                      dim3(256), 0, st, a);
   if (a.splits > 1) return launch_merge<T, DP, kTile, 16 * NQ, 4>(a, st);

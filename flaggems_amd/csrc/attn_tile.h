@@ -330,7 +330,7 @@ template <typename T, int FMT, int DP, int NQ>
 int launch_tile(const CacheAttnArgs& a, hipStream_t st) {
   const FgFlashParams& p = a.p.base;
   const int64_t blocks = fg_cdiv((int64_t)a.max_q * a.group, 64 * NQ) * a.splits * 8 * fg_cdiv((int64_t)p.batch * p.Hk, 8);
-  FG_REQUIRE(blocks < ((int64_t)1 << 31), FG_ERR_UNSUPPORTED, "cache_attn_fwd: too many query rows for one launch");
+  FG_REQUIRE(blocks < kMostBlocks, FG_ERR_UNSUPPORTED, "cache_attn_fwd: too many query rows for one launch");
   if (a.page_bits >= 0)
     hipLaunchKernelGGL((attn_tile_kernel<T, FMT, DP, true, NQ>), dim3((unsigned)blocks), dim3(256), 0, st, a);
   else

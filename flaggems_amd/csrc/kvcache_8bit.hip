@@ -13,6 +13,7 @@
 namespace {
 
 enum { kE4M3 = FG_CACHE_E4M3, kE5M2 = FG_CACHE_E5M2 };
+constexpr int64_t kMostBlocks = (int64_t)1 << 24;  // of 256 threads: a launch counts threads in 32 bits
 
 template <int FMT> struct Fp8;
 template <> struct Fp8<kE4M3> {
@@ -41,13 +42,14 @@ template <> struct Fp8<kE5M2> {
 // (the residual x - q * s is exact in one fused operation, so q' is x / s with a relative error of 2^-46 in front of its one
 // rounding: a quotient that is an fp32 number, such as a middle between two 8-bit ones, comes out as it is).  x is cut to
 // twice the range first, so that nothing overflows.  Seven plain operations an element instead of the eighteen of a division, which
-// alone would keep the vector ALU busy for 40 of the 76 us below.  Scales outside [2^-100, 2^100] are divided by.
+// alone would keep the vector ALU busy for 40 of the 76 us below.  Scales outside [2^-60, 2^100] are divided by (the residual of a
+// smaller one would lose bits below 2^-149).
 template <int FMT> struct Quotient {
   float s, r, most;
   bool plain;
   __device__ __forceinline__ explicit Quotient(float scale) : s(scale), r(1.0f / scale) {
     const float a = fabsf(scale);
-    plain = a >= 0x1p-100f && a <= 0x1p100f;     // false for NaN
+    plain = a >= 0x1p-60f && a <= 0x1p100f;     // false for NaN
     most = 2.0f * Fp8<FMT>::kMax * a;
   }
   __device__ __forceinline__ float operator()(float x) const {
@@ -139,7 +141,9 @@ __global__ __launch_bounds__(256) void cache_write8_kernel(WriteArgs a) {
 template <typename T, int FMT, int CH>
 int write_launch(WriteArgs a, int slot_is_i64, hipStream_t st) {
   a.waves_log2 = a.row > 256 * CH ? 2 : (a.row > 128 * CH ? 1 : 0);
-  const unsigned grid = (unsigned)fg_cdiv((a.num_tokens * 2) << a.waves_log2, 4);
+  const int64_t grid64 = fg_cdiv((a.num_tokens * 2) << a.waves_log2, 4);
+  FG_REQUIRE(grid64 < kMostBlocks, FG_ERR_UNSUPPORTED, "reshape_and_cache_flash_8bit: problem too large for one launch");
+  const unsigned grid = (unsigned)grid64;
   if (slot_is_i64) hipLaunchKernelGGL((cache_write8_kernel<T, FMT, CH, int64_t>), dim3(grid), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((cache_write8_kernel<T, FMT, CH, int32_t>), dim3(grid), dim3(256), 0, st, a);
   return fg_check_launch("reshape_and_cache_flash_8bit");
@@ -257,6 +261,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(ReadArgs a) {
 
 template <typename U, int FMT, int CH>
 int read_launch(const ReadArgs& a, hipStream_t st) {
+  FG_REQUIRE(fg_cdiv(a.num_rows, 4) < kMostBlocks, FG_ERR_UNSUPPORTED, "gather_cache_flash: problem too large for one launch");
   hipLaunchKernelGGL((cache_read_kernel<U, FMT, CH>), dim3((unsigned)fg_cdiv(a.num_rows, 4)), dim3(256), 0, st, a);
   return fg_check_launch("gather_cache_flash");
 }
@@ -341,8 +346,8 @@ extern "C" int fg_gather_cache_flash(const void* key_cache, const void* value_ca
   if (num_rows == 0 || batch == 0 || (int64_t)H * D == 0) return FG_OK;
   FG_REQUIRE(key_cache && value_cache && key && value && block_table && cu_seqlens, FG_ERR_INVALID,
              "gather_cache_flash: null pointer");
-  FG_REQUIRE((int64_t)H * D < ((int64_t)1 << 30) && num_rows < ((int64_t)1 << 32), FG_ERR_UNSUPPORTED,
-             "gather_cache_flash: problem too large for one launch");
+  FG_REQUIRE((int64_t)H * D < ((int64_t)1 << 30), FG_ERR_UNSUPPORTED, "gather_cache_flash: problem too large for one launch");
+  FG_REQUIRE(num_pages > 0, FG_ERR_INVALID, "gather_cache_flash: the cache has no pages");  // (there is nothing that could be read)
   FG_REQUIRE(key_page_stride >= (int64_t)page_size * H * D && value_page_stride >= (int64_t)page_size * H * D, FG_ERR_INVALID,
              "gather_cache_flash: page stride smaller than a page (%d x %d x %d)", page_size, H, D);
   FG_REQUIRE(key_stride >= (int64_t)H * D && value_stride >= (int64_t)H * D, FG_ERR_INVALID,

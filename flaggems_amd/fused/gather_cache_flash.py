@@ -27,7 +27,7 @@ def gather_cache_flash(
     A cache of fp16, bf16 or fp32 is copied (dtype, if given, is its own).  An 8-bit cache (see reshape_and_cache_flash) is
     read as cache * scale, rounded once to `dtype` (bf16 if neither dtype nor outputs are given).  key / value, if given,
     are written and returned; rows that belong to no sequence are left as they were.  A position whose page is not in the
-    table, or not in the cache, gives zeros."""
+    table, or not in the cache (which has one page at least), gives zeros."""
     logger.debug("GEMS GATHER_CACHE_FLASH")
     num_blocks, block_size, num_heads, head_size = key_cache.shape
     batch = cu_seqlens.size(0) - 1
@@ -43,6 +43,7 @@ def gather_cache_flash(
     assert cu_seqlens.dtype is torch.int32 and batch >= 0 and cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous int32 [batch + 1]"
     if seq_starts is not None:
         assert seq_starts.dtype is torch.int32 and seq_starts.is_contiguous() and seq_starts.shape == (batch,), "seq_starts must be contiguous int32 [batch]"
+    assert key_cache.is_cuda, "the tensors must be on a GPU"
     fmt = _C.cache_format(cache_dtype, kv_cache_dtype)
     if dtype is None:
         dtype = key.dtype if key is not None else torch.bfloat16 if fmt is not None else cache_dtype

@@ -60,6 +60,7 @@ def _quantize_and_cache(key, value, key_cache, value_cache, slot_mapping, kv_cac
     assert value_cache.dtype is cache_dtype and value.dtype is dtype, "key/value and their caches must match"
     assert cache_heads == num_heads and cache_size == head_size and value_cache.shape == key_cache.shape, "cache shape"
     assert v_heads == num_heads and v_size == head_size and rows >= num_tokens <= v_rows, "key/value shape"
+    assert key.is_cuda, "the tensors must be on a GPU"
     assert slot_dtype is torch.int64 or slot_dtype is torch.int32, "slot_mapping must be int64 or int32"
     assert num_tokens <= 1 or slot_mapping.stride(0) == 1, "slot_mapping must be contiguous"
     token, page = (head_size, 1), (num_heads * head_size, head_size, 1)

@@ -243,8 +243,12 @@ def test_c_entry_points_refuse_on_the_host():
 
     assert read(rows=0) == 0 and read(batch=0) == 0
     for kw, word in (({"rows": -1}, "negative"), ({"ps": 0}, "page size"), ({"dtype": 9}, "dtype"), ({"fmt": 3}, "format"), ({"ptr": None}, "null"),
-                     ({"kps": 2047}, "page stride"), ({"ks": 127}, "row stride"), ({"vs": 0}, "row stride"), ({"ss": 5}, "scale")):
+                     ({"kps": 2047}, "page stride"), ({"ks": 127}, "row stride"), ({"vs": 0}, "row stride"), ({"ss": 5}, "scale"),
+                     ({"pages": 0}, "no pages")):
         assert read(**kw) == -1 and word in _C.last_error(), kw
+
+    assert write(n=1 << 27) == -2 and "too large" in _C.last_error()
+    assert read(rows=1 << 27) == -2 and "too large" in _C.last_error()
 
     def attn(**kw):
         c = _C.FgCacheAttnParams()
@@ -267,7 +271,9 @@ def test_c_entry_points_refuse_on_the_host():
                          ({"q": None}, -1, "null"), ({"D": 72}, -1, "multiple of 16"), ({"D": 272}, -1, "at most 256"), ({"Hq": 7}, -1, "not a multiple"),
                          ({"page_size": 0}, -1, "page size"), ({"max_seqlen_q": 0}, -1, "max_seqlen_q"), ({"num_pages": 0}, -1, "pages"),
                          ({"alibi_slopes": 256}, -2, "alibi"), ({"k_cache": 264}, -2, "aligned"), ({"k_row_stride": 136}, -2, "aligned"),
-                         ({"v_page_stride": 2056}, -2, "aligned"), ({"q_head_stride": 66}, -2, "aligned"), ({"batch": 65536}, -2, "grid")):
+                         ({"v_page_stride": 2056}, -2, "aligned"), ({"q_head_stride": 66}, -2, "aligned"), ({"batch": 65536}, -2, "grid"),
+                         ({"table_width": 1 << 27}, -2, "spans"), ({"total_q": 1 << 30, "max_seqlen_q": 1 << 30}, -2, "too many"),
+                         ({"total_q": 1 << 30, "max_seqlen_q": 1 << 30, "D": 256}, -2, "too many")):
         assert attn(**kw) == rc and word in _C.last_error(), (kw, _C.last_error())
 
 
@@ -360,3 +366,31 @@ def test_bounds_beyond_32_bits_are_cut(calls):
     a, b = (_C.FgCacheAttnParams.from_buffer_copy(c[0]) for n, c in calls.rec.calls if n == "fg_cache_attn_fwd")
     assert (a.base.window_left, a.base.window_right, a.num_sink_tokens) == (2 ** 31 - 1,) * 3
     assert (b.base.window_left, b.base.window_right, b.num_sink_tokens) == (-1, -1, 0)
+
+
+def test_tensors_off_the_gpu_are_refused():
+    kc, vc = cache()
+    x = torch.randn(7, 2, 64).half()
+    with pytest.raises(AssertionError, match="on a GPU"):
+        flag_gems.reshape_and_cache_flash(x, x, kc, vc, torch.arange(7), "fp8", None, None)
+    with pytest.raises(AssertionError, match="on a GPU"):
+        flag_gems.gather_cache_flash(kc, vc, torch.zeros(1, 2, dtype=torch.int32), torch.tensor([0, 7], dtype=torch.int32), 7)
+    with pytest.raises(AssertionError):
+        attend(kc, vc)
+
+
+def test_scratch_goes_by_the_tokens_that_are_there():
+    """A bound on the sequences' length that is far above the number of tokens costs nothing."""
+    def scratch(total, longest):
+        c = _C.FgCacheAttnParams()
+        p = c.base
+        for f in ("q", "k_cache", "v_cache", "out", "cu_seqlens_q", "seqused_k", "block_table"):
+            setattr(p, f, 256)
+        p.total_q, p.batch, p.Hq, p.Hk, p.D, p.page_size, p.max_seqlen_q, p.max_seqlen_k = total, 1, 8, 2, 256, 16, longest, 20000
+        for n in "kv":
+            setattr(p, n + "_page_stride", 8192), setattr(p, n + "_row_stride", 512), setattr(p, n + "_head_stride", 256)
+        p.dtype, p.window_left, p.window_right = _C.FG_BF16, -1, -1
+        c.cache_format, c.num_pages, c.table_width = _C.CACHE_E4M3, 6, 1250
+        return _C.lib().fg_cache_attn_workspace_bytes(ctypes.byref(c), 0)
+
+    assert scratch(1, 1) > 0 and scratch(1, 2 ** 31 - 1) == scratch(1, 1)

@@ -88,6 +88,23 @@ def test_write_8bit_every_value_and_ties(gpu, fmt):
     assert torch.isnan(values(kc)[0]).all() and not torch.isnan(values(kc)[1:]).any()
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("scale", [1.375 * 2.0 ** -99, 1.375 * 2.0 ** -61, 1.375 * 2.0 ** -60, 1.375 * 2.0 ** 99, 1.375 * 2.0 ** 101])
+def test_write_8bit_ties_at_extreme_scales(gpu, fmt, scale):
+    """Middles between neighbours times a scale of four bits are fp32 numbers: their quotients are exact, and go to the even one."""
+    codes = torch.arange(256, dtype=torch.uint8).view(FMT[fmt]).float()
+    v = torch.unique(codes[torch.isfinite(codes)])
+    x = torch.cat([v, (v[1:] + v[:-1]) / 2])
+    x = torch.cat([x, torch.zeros(-x.numel() % 16)]).view(-1, 1, 16)
+    scaled = (x.double() * scale).float()
+    assert torch.equal(scaled.double(), x.double() * scale)
+    kc = torch.zeros(x.shape[0], 1, 1, 16, dtype=FMT[fmt], device=gpu); vc = torch.zeros_like(kc)
+    s = torch.tensor(scale, device=gpu)
+    flag_gems.reshape_and_cache_flash(scaled.to(gpu), scaled.to(gpu), kc, vc, torch.arange(x.shape[0], device=gpu), "fp8_" + fmt, s, s)
+    want = O.round_to_8bit(x.double(), fmt)
+    assert torch.equal(values(kc).view(-1), want.view(-1)) and torch.equal(values(vc).view(-1), want.view(-1))
+
+
 def test_write_8bit_nothing(gpu):
     kc = dirty((2, 4, 2, 16), "e4m3", gpu); vc = kc.clone(); old = kc.clone()
     x = torch.ones(0, 2, 16, device=gpu, dtype=torch.float16)
