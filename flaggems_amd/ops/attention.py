@@ -142,6 +142,7 @@ def mha_varlan_fwd(
 
 
 # Scratch sizes by everything they depend on: sizes, masks and the device (one library call less for a shape seen before).
+# Kept of calls that ran only: the library also answers 0 for parameters that it refuses, for reasons that are not in the key.
 _cache_attn_scratch = {}
 _INT32_MAX = 2 ** 31 - 1
 
@@ -211,13 +212,14 @@ def cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, page_table, alibi_slop
         ws_bytes = _cache_attn_scratch.get(key)
         if ws_bytes is None:
             ws_bytes = _C.lib().fg_cache_attn_workspace_bytes(packed(0, 0), index)
-            if len(_cache_attn_scratch) >= 4096:
-                _cache_attn_scratch.clear()
-            _cache_attn_scratch[key] = ws_bytes
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes > 0 else None
         rc = _C.lib().fg_cache_attn_fwd(packed(0 if ws is None else ws.data_ptr(), ws_bytes), _C.current_stream(device))
         if rc:
             _C.check(rc, "fg_cache_attn_fwd")
+        if key not in _cache_attn_scratch:
+            if len(_cache_attn_scratch) >= 4096:
+                _cache_attn_scratch.clear()
+            _cache_attn_scratch[key] = ws_bytes
     return out, lse
 
 
