@@ -70,6 +70,13 @@ struct Plan {
   size_t stream_bytes, tile_bytes;  // scratch for the key ranges; one after the other
 };
 
+// Most scratch for the key ranges of chunks: their partial results grow with the tokens of the call (1.5 GiB for 16384 tokens of 32
+// heads of 128 in 6 ranges) and lie next to a cache that may fill the card.  1 GiB keeps the speed where it was measured: 8 chunks of up to
+// 4096 tokens over up to 131072 keys 24.2 ms in 3 ranges, 24.0 in 6, 46.4 unsplit (row blocks of sequences of different length start at
+// different times, and no longer share what the L2 holds); one of 8200 over 131072 18.4 ms in 3, 18.3 in 9, 21.0 unsplit.  The
+// stream kernel's ranges need no bound: there are some for fewer than 512 row blocks only, and then at most 52 MB.
+constexpr size_t kMostScratch = (size_t)1 << 30;
+
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 
 // Microseconds that a launch of the tile kernel takes with row blocks of 64 * nq rows and `splits` key ranges, from what was
@@ -140,7 +147,7 @@ Plan make_plan(const FgCacheAttnParams& c) {
       // even: exact; otherwise half a block is left over in a sequence on average
       const int64_t blocks = p.Hk * (even ? fg_cdiv((int64_t)p.max_seqlen_q * G, rows) * p.batch : (int64_t)p.total_q * G / rows + p.batch / 2 + 1);
       const int64_t tiles = fg_cdiv(keys_of(fg_cdiv(rows, G), kTileKeys), kTileKeys);
-      for (int splits = 1; splits <= 64 && (splits == 1 || tiles >= 2 * splits); ++splits) {
+      for (int splits = 1; splits <= 64 && (splits == 1 || (tiles >= 2 * splits && splits * row * p.total_q <= kMostScratch)); ++splits) {
         const double us = tile_cost(blocks, (double)tiles, nq, dp, cus, splits, even, (double)row * (double)p.total_q);
         if (plan.tile_splits == 0 || us < best) best = us, plan.tile_nq = nq, plan.tile_splits = splits;
       }

@@ -64,3 +64,36 @@ def test_a_refused_call_leaves_no_answer_behind(asked):
     attend(0)
     refused, first, second = scratch_of(asked)
     assert refused == 0 and first == second > 0
+
+
+def sizes(total, batch, longest, keys, hq=32, hk=8, dim=128, window=-1, sinks=0, page=16, fmt=_C.CACHE_E4M3, **kw):
+    """The parameters of a causal call, with addresses that no kernel will see."""
+    c = _C.FgCacheAttnParams()
+    p = c.base
+    for f in ("q", "k_cache", "v_cache", "out", "cu_seqlens_q", "seqused_k", "block_table"):
+        setattr(p, f, 256)
+    p.total_q, p.batch, p.Hq, p.Hk, p.D, p.page_size, p.max_seqlen_q, p.max_seqlen_k = total, batch, hq, hk, dim, page, longest, keys
+    p.q_row_stride = p.o_row_stride = hq * dim
+    p.q_head_stride = p.o_head_stride = dim
+    for n in "kv":
+        setattr(p, n + "_page_stride", page * hk * dim), setattr(p, n + "_row_stride", hk * dim), setattr(p, n + "_head_stride", dim)
+    p.dtype, p.window_left, p.window_right, p.is_causal, p.softmax_scale, p.block_table_stride = _C.FG_BF16, window, -1, 1, 0.1, -(-keys // page)
+    c.cache_format, c.num_pages, c.table_width, c.num_sink_tokens = fmt, 1 << 20, -(-keys // page), sinks
+    for name, value in kw.items():
+        setattr(c if hasattr(c, name) else p, name, value)
+    return c
+
+
+@pytest.mark.parametrize("hq,hk,dim", [(32, 8, 128), (64, 8, 128), (128, 1, 64), (8, 8, 64), (32, 4, 256)])
+def test_scratch_stays_small(hq, hk, dim):
+    """1 GiB for the ranges of chunks and 52 MB for those of few tokens, whatever the batch: total * (DP + 2) * 4 bytes a range
+    and query head."""
+    most = 0
+    for total in [1, 3, 40, 333, 1000, 2047, 4096, 5001, 8192, 8200, 12000, 16384, 33000, 33279, 100003]:
+        for batch in (1, 2, 8, 63, 512):
+            for keys in (1, 700, 8192, 131072, 1 << 20):
+                for longest in {total, max(1, total // batch), min(total, 4096)}:
+                    for window in (-1, 4095):
+                        c = sizes(total, batch, longest, keys, hq, hk, dim, window, 4)
+                        most = max(most, _C.lib().fg_cache_attn_workspace_bytes(ctypes.byref(c), 0))
+    assert 0 < most <= (1 << 30) + 52_000_000
