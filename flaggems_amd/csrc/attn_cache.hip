@@ -65,6 +65,7 @@ struct Plan {
   int stream_q;     // sequences with up to so many new tokens take the stream kernel (0: none)
   bool tile;        // the others take the tile kernel
   int nq, tile_nq;  // 16-row tiles of a row block (stream), of a wave (tile)
+  int tile_batch;   // sequences of a launch of the tile kernel (0: one of them alone is too long for one)
   int pages;        // stream kernel: how pages are found
   int splits, min_tiles, tile_splits, tile_min_tiles;
   size_t stream_bytes, tile_bytes;  // scratch for the key ranges; one after the other
@@ -148,9 +149,16 @@ Plan make_plan(const FgCacheAttnParams& c) {
       const int64_t blocks = p.Hk * (even ? fg_cdiv((int64_t)p.max_seqlen_q * G, rows) * p.batch : (int64_t)p.total_q * G / rows + p.batch / 2 + 1);
       const int64_t tiles = fg_cdiv(keys_of(fg_cdiv(rows, G), kTileKeys), kTileKeys);
       for (int splits = 1; splits <= 64 && (splits == 1 || (tiles >= 2 * splits && splits * row * p.total_q <= kMostScratch)); ++splits) {
+        if (tile_blocks(p, p.max_seqlen_q, nq, splits, p.batch) >= kMostBlocks) break;
         const double us = tile_cost(blocks, (double)tiles, nq, dp, cus, splits, even, (double)row * (double)p.total_q);
         if (plan.tile_splits == 0 || us < best) best = us, plan.tile_nq = nq, plan.tile_splits = splits;
       }
+    }
+    plan.tile_batch = p.batch;
+    if (plan.tile_splits == 0) {  // more than a launch holds in any cut: unsplit, a few sequences at a time
+      plan.tile_nq = 2, plan.tile_splits = 1;
+      const int64_t eights = (kMostBlocks - 1) / tile_blocks(p, p.max_seqlen_q, 2, 1, 1) * fg_cdiv(p.Hk, 8);
+      plan.tile_batch = (int)(eights * 8 / p.Hk);
     }
     plan.tile_min_tiles = 2;
     if (plan.tile_splits > 1) plan.tile_bytes = plan.tile_splits * row * p.total_q;
@@ -229,6 +237,7 @@ extern "C" int fg_cache_attn_fwd(const FgCacheAttnParams* c, void* stream) {
   a.page_bits = ((int64_t)1 << s) == p.page_size ? s : -1;
   const Plan plan = make_plan(a.p);
   const bool scratch = p.workspace != nullptr && fg_aligned(p.workspace, 16) && (size_t)p.workspace_bytes >= plan.stream_bytes + plan.tile_bytes;
+  FG_REQUIRE(!plan.tile || plan.tile_batch > 0, FG_ERR_UNSUPPORTED, "cache_attn_fwd: too many query rows for one launch");
   const int dp = padded_dim(p.D);
   hipStream_t st = (hipStream_t)stream;
   if (plan.stream_q > 0) {
@@ -251,5 +260,17 @@ extern "C" int fg_cache_attn_fwd(const FgCacheAttnParams* c, void* stream) {
   a.part_rows = p.total_q;
   a.part_o = (float*)((char*)p.workspace + plan.stream_bytes);
   a.part_ml = a.part_o + (size_t)a.splits * a.part_rows * p.Hq * dp;
-  return p.dtype == FG_F16 ? tile_formats<f16_t>(a, plan.tile_nq, st) : tile_formats<bf16_t>(a, plan.tile_nq, st);
+  const int batch = p.batch;
+  for (int b = 0; b < batch; b += plan.tile_batch) {
+    CacheAttnArgs s = a;
+    s.p.base.batch = std::min(plan.tile_batch, batch - b);
+    s.p.base.cu_seqlens_q += b;
+    s.p.base.seqused_k += b;
+    s.p.base.block_table += b * p.block_table_stride;
+    if (s.p.k_scale != nullptr) s.p.k_scale += b * s.p.k_scale_batch_stride;
+    if (s.p.v_scale != nullptr) s.p.v_scale += b * s.p.v_scale_batch_stride;
+    const int done = p.dtype == FG_F16 ? tile_formats<f16_t>(s, plan.tile_nq, st) : tile_formats<bf16_t>(s, plan.tile_nq, st);
+    if (done != FG_OK) return done;
+  }
+  return FG_OK;
 }

@@ -332,10 +332,15 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(CacheAttnArgs a) {
   }
 }
 
+// Workgroups of a launch for `batch` sequences with up to max_q new tokens.
+inline int64_t tile_blocks(const FgFlashParams& p, int64_t max_q, int nq, int splits, int64_t batch) {
+  return fg_cdiv(max_q * (p.Hq / p.Hk), 64 * nq) * splits * 8 * fg_cdiv(batch * p.Hk, 8);
+}
+
 template <typename T, int FMT, int DP, int NQ>
 int launch_tile(const CacheAttnArgs& a, hipStream_t st) {
   const FgFlashParams& p = a.p.base;
-  const int64_t blocks = fg_cdiv((int64_t)a.max_q * a.group, 64 * NQ) * a.splits * 8 * fg_cdiv((int64_t)p.batch * p.Hk, 8);
+  const int64_t blocks = tile_blocks(p, a.max_q, NQ, a.splits, p.batch);
   FG_REQUIRE(blocks < kMostBlocks, FG_ERR_UNSUPPORTED, "cache_attn_fwd: too many query rows for one launch");
   if (a.page_bits >= 0)
     hipLaunchKernelGGL((attn_tile_kernel<T, FMT, DP, true, NQ>), dim3((unsigned)blocks), dim3(256), 0, st, a);

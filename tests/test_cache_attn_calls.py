@@ -97,3 +97,59 @@ def test_scratch_stays_small(hq, hk, dim):
                         c = sizes(total, batch, longest, keys, hq, hk, dim, window, 4)
                         most = max(most, _C.lib().fg_cache_attn_workspace_bytes(ctypes.byref(c), 0))
     assert 0 < most <= (1 << 30) + 52_000_000
+
+
+@pytest.fixture(scope="module")
+def launched(tmp_path_factory):
+    """launched([parameters, ...]): for each call (return code, message, launches), with the scratch that it asks for."""
+    import json
+    import os
+    import subprocess
+    import sys
+
+    from flaggems_amd import _C
+
+    where = str(tmp_path_factory.mktemp("recorded"))
+    script = os.path.join(os.path.dirname(os.path.abspath(__file__)), "emu", "recorded.py")
+
+    def record(calls):
+        for c in calls:
+            c.base.workspace_bytes = _C.lib().fg_cache_attn_workspace_bytes(ctypes.byref(c), 0)
+            c.base.workspace = 1 << 20 if c.base.workspace_bytes else 0
+        spec = [["fg_cache_attn_fwd", bytes(c).hex()] for c in calls]
+        run = subprocess.run([sys.executable, script, _C.LIB_PATH, where], input=json.dumps(spec), stdout=subprocess.PIPE, text=True, check=True, timeout=300)
+        return [(rc, text, [(name, grid, block, _C.FgCacheAttnParams.from_buffer_copy(bytes.fromhex(arg))) for name, grid, block, arg in launches])
+                for rc, text, launches in json.loads(run.stdout)]
+
+    return record
+
+
+UNEVEN = [dict(total=longest + batch - 1, batch=batch, longest=longest, keys=keys, hq=hq, hk=hk, dim=dim)
+          for hq, hk, dim in [(64, 8, 128), (8, 8, 64), (16, 1, 64), (32, 8, 128)] for batch in (1, 64, 512, 4096, 65535)
+          for longest in (1000, 32768, 131072, 1 << 20) for keys in (1 << 14, 1 << 20)]
+
+
+def test_one_long_chunk_among_many_sequences(launched):
+    """Grids go by the number of sequences times the longest.  Where that is more than a launch holds, sequences are launched a
+    few at a time: no call is refused, and every sequence is in one launch of each kernel that it may need."""
+    calls = [sizes(k_scale=1 << 21, v_scale=1 << 22, k_scale_batch_stride=3, v_scale_batch_stride=5, **kw) for kw in UNEVEN]
+    several = 0
+    for kw, c, (rc, text, launches) in zip(UNEVEN, calls, launched(calls)):
+        assert rc == 0, (kw, text)
+        assert launches and all(g * b < 1 << 32 for _, grid, block, _ in launches for g, b in zip(grid, block)), kw
+        tiles = [a for name, _, _, a in launches if "attn_tile_kernel" in name]
+        several += len(tiles) > 1
+        at = 0
+        for a in tiles:
+            assert (a.base.cu_seqlens_q, a.base.seqused_k) == (256 + 4 * at, 256 + 4 * at)
+            assert a.base.block_table == 256 + 4 * at * c.base.block_table_stride
+            assert (a.k_scale, a.v_scale) == ((1 << 21) + 12 * at, (1 << 22) + 20 * at)
+            at += a.base.batch
+        assert at == kw["batch"], kw
+    assert several > 10
+
+
+def test_refusals_come_before_any_launch(launched):
+    """A single sequence with more row blocks than a launch holds: neither kernel runs."""
+    (rc, text, launches), = launched([sizes(total=(1 << 29) + 1, batch=2, longest=1 << 29, keys=1 << 14)])
+    assert rc == -2 and "too many" in text and not launches

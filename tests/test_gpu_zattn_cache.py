@@ -294,3 +294,29 @@ def test_custom_op_takes_an_8bit_cache(gpu):
     out, lse = torch.ops.flag_gems.flash_attn_varlen_func(q, kc, vc, 5, cu, 300, None, used, None, 0.0, 0.125, True, [-1, -1], 0.0, None, False,
                                                           False, table, True, None, None, None, ks, vs, 2)
     assert_close(out, lse, O.cache_attention(q, kc, vc, cu, used, table, 0.125, k_scale=ks, v_scale=vs), torch.bfloat16, 64)
+
+
+def test_more_sequences_than_a_launch_holds(gpu):
+    """65535 sequences, one of them a chunk: the chunk kernel takes them in two launches.  Checked against the oracle: the chunk, the
+    sequences where the launches meet and the last ones, each a call of the oracle of its own."""
+    batch, n, heads, dim = 65535, 520, 64, 64
+    g = torch.Generator(device=gpu).manual_seed(3)
+    keys = torch.ones(batch, dtype=torch.int32, device=gpu)
+    new = torch.ones(batch, dtype=torch.int32, device=gpu)
+    at = 40000
+    keys[at], new[at] = 600, n
+    cu = torch.cat([torch.zeros(1, dtype=torch.int32, device=gpu), new.cumsum(0, dtype=torch.int32)])
+    kc, vc = (torch.randn(2048, 1, heads, dim, generator=g, device=gpu).mul(20).to(torch.float8_e4m3fn) for _ in range(2))
+    table = torch.randint(0, 2048, (batch, 600), generator=g, device=gpu, dtype=torch.int32)
+    q = torch.randn(int(cu[-1]), heads, dim, generator=g, device=gpu).to(torch.bfloat16)
+    ks, vs = (torch.rand(batch, 1, generator=g, device=gpu) * 0.04 + 0.03 for _ in range(2))
+    out, lse = flag_gems.flash_attn_varlen_func(q, kc, vc, n, cu, 600, seqused_k=keys, causal=True, block_table=table, return_softmax_lse=True,
+                                                k_descale=ks, v_descale=vs)
+    meet = ((1 << 24) - 1) // (5 * 8) * 8 // heads                    # sequences of the first launch
+    assert 0 < meet < batch
+    for first, last in ((0, 2), (at, at + 1), (meet - 2, meet + 2), (batch - 2, batch)):
+        a, b = int(cu[first]), int(cu[last])
+        ref = O.cache_attention(q[a:b], kc, vc, cu[first:last + 1] - a, keys[first:last], table[first:last], dim ** -0.5, k_scale=ks[first:last],
+                                v_scale=vs[first:last])
+        assert_close(out[a:b], lse[:, a:b], ref, torch.bfloat16, dim)
+    assert not torch.isnan(out).any()
