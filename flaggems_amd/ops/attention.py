@@ -212,8 +212,13 @@ def cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, page_table, alibi_slop
         ws_bytes = _cache_attn_scratch.get(key)
         if ws_bytes is None:
             ws_bytes = _C.lib().fg_cache_attn_workspace_bytes(packed(0, 0), index)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes > 0 else None
-        rc = _C.lib().fg_cache_attn_fwd(packed(0 if ws is None else ws.data_ptr(), ws_bytes), _C.current_stream(device))
+        ws = None
+        if ws_bytes > 0:
+            try:
+                ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+            except torch.OutOfMemoryError:  # up to 1 GiB: the call runs without it, unsplit
+                pass
+        rc = _C.lib().fg_cache_attn_fwd(packed(0, 0) if ws is None else packed(ws.data_ptr(), ws_bytes), _C.current_stream(device))
         if rc:
             _C.check(rc, "fg_cache_attn_fwd")
         if key not in _cache_attn_scratch:

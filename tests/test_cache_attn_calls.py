@@ -153,3 +153,29 @@ def test_refusals_come_before_any_launch(launched):
     """A single sequence with more row blocks than a launch holds: neither kernel runs."""
     (rc, text, launches), = launched([sizes(total=(1 << 29) + 1, batch=2, longest=1 << 29, keys=1 << 14)])
     assert rc == -2 and "too many" in text and not launches
+
+
+def test_a_full_card_costs_the_ranges_only(asked, monkeypatch):
+    """No memory for the scratch: the call runs without, and the next one of these sizes asks again."""
+    from flaggems_amd.ops import attention
+
+    class Full:
+        full = True
+
+        def empty(self, *size, **kw):
+            if self.full and kw["dtype"] is torch.uint8:
+                raise torch.OutOfMemoryError("no room")
+            return torch.empty(*size, **kw)
+
+        def __getattr__(self, name):
+            return getattr(torch, name)
+
+    card = Full()
+    monkeypatch.setattr(attention, "torch", card)
+    kc, vc = torch.zeros(2, 6, 16, 8, 128).to(E4M3).unbind(0)
+    cu, used = torch.arange(4, dtype=torch.int32), torch.full((3,), 50, dtype=torch.int32)
+    q = torch.randn(3, 32, 128).bfloat16()
+    for card.full in (True, False, True):
+        flag_gems.flash_attn_varlen_func(q, kc, vc, 1, cu, 131072, seqused_k=used, causal=True, block_table=torch.zeros(3, 8192, dtype=torch.int32))
+    without, given, again = scratch_of(asked)
+    assert without == again == 0 < given
