@@ -242,7 +242,7 @@ def cache_format(cache_dtype, kv_cache_dtype="auto"):
             raise ValueError("a cache of bytes needs kv_cache_dtype fp8, fp8_e4m3 or fp8_e5m2, got %r" % (kv_cache_dtype,))
         return _CACHE_NAMES[kv_cache_dtype]
     fmt = _CACHE_FORMAT.get(cache_dtype)
-    if fmt is not None and _CACHE_NAMES.get(kv_cache_dtype, fmt) != fmt:
+    if fmt is not None and kv_cache_dtype != "auto" and _CACHE_NAMES.get(kv_cache_dtype) != fmt:
         raise ValueError("kv_cache_dtype %r does not fit a cache of %s" % (kv_cache_dtype, cache_dtype))
     return fmt
 

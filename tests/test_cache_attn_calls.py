@@ -179,3 +179,17 @@ def test_a_full_card_costs_the_ranges_only(asked, monkeypatch):
         flag_gems.flash_attn_varlen_func(q, kc, vc, 1, cu, 131072, seqused_k=used, causal=True, block_table=torch.zeros(3, 8192, dtype=torch.int32))
     without, given, again = scratch_of(asked)
     assert without == again == 0 < given
+
+
+@pytest.mark.parametrize("name", ["int8", "fp8_inc", "fp8_ds_mla", "e4m3", "FP8", "", None])
+def test_names_of_no_format_are_refused(asked, name):
+    """Not taken for what the cache's own type would be."""
+    x, slots = torch.randn(7, 2, 64).half(), torch.arange(7)
+    table, cu = torch.zeros(3, 4, dtype=torch.int32), torch.tensor([0, 5, 5, 30], dtype=torch.int32)
+    for kind in (E4M3, E5M2, torch.uint8):
+        c = torch.zeros(6, 16, 2, 64).to(kind)
+        with pytest.raises(ValueError, match="kv_cache_dtype"):
+            flag_gems.reshape_and_cache_flash(x, x, c, c.clone(), slots, name, None, None)
+        with pytest.raises(ValueError, match="kv_cache_dtype"):
+            flag_gems.gather_cache_flash(c, c, table, cu, 30, name)
+    assert not asked.calls
