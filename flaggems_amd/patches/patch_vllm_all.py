@@ -81,6 +81,10 @@ def custom_gems_write_to_paged_cache(key, value, key_cache, value_cache, slot_ma
     reshape_and_cache(key, value, key_cache, value_cache, slot_mapping.flatten(), kv_cache_dtype, k_scale, v_scale)
 
 
+# the element types of caches that vLLM hands over as bytes, by kv_cache_dtype
+_FP8_TYPES = {"fp8": torch.float8_e4m3fn, "fp8_e4m3": torch.float8_e4m3fn, "fp8_e5m2": torch.float8_e5m2}
+
+
 def custom_gems_flash_attention_impl_forward(
     self,
     layer: torch.nn.Module,
@@ -104,12 +108,15 @@ def custom_gems_flash_attention_impl_forward(
     if attn_metadata is None:  # memory-profiling pass
         return output
     quantized = self.kv_cache_dtype.startswith("fp8")
-    if quantized and getattr(kv_cache, "dtype", None) not in _C.CACHE_8BIT:
-        raise NotImplementedError("kv_cache_dtype %s needs a cache of 8-bit elements" % self.kv_cache_dtype)
+    if quantized:
+        if self.kv_cache_dtype not in _FP8_TYPES:
+            raise NotImplementedError("kv_cache_dtype %s is not supported for FlashAttentionImpl" % self.kv_cache_dtype)
+        if getattr(kv_cache, "dtype", None) not in _C.CACHE_8BIT:
+            raise NotImplementedError("kv_cache_dtype %s needs a cache of 8-bit elements" % self.kv_cache_dtype)
+        if kv_cache.dtype == torch.uint8:
+            kv_cache = kv_cache.view(_FP8_TYPES[self.kv_cache_dtype])
 
     n = attn_metadata.num_actual_tokens
-    if quantized and kv_cache.dtype == torch.uint8:
-        kv_cache = kv_cache.view(torch.float8_e5m2 if self.kv_cache_dtype == "fp8_e5m2" else torch.float8_e4m3fn)
     key_cache, value_cache = kv_cache.unbind(0)
     reshape_and_cache_flash(
         key, value, key_cache, value_cache, attn_metadata.slot_mapping, self.kv_cache_dtype,

@@ -193,3 +193,26 @@ def test_names_of_no_format_are_refused(asked, name):
         with pytest.raises(ValueError, match="kv_cache_dtype"):
             flag_gems.gather_cache_flash(c, c, table, cu, 30, name)
     assert not asked.calls
+
+
+@pytest.mark.parametrize("name", ["fp8_inc", "fp8_ds_mla", "fp8e4"])
+@pytest.mark.parametrize("kind", [torch.uint8, E4M3])
+def test_vllm_hook_refuses_caches_it_does_not_know(monkeypatch, name, kind):
+    """kv_cache_dtype names that begin with fp8 and stand for another layout or number format: refused, nothing written."""
+    import importlib
+    import types
+
+    from flaggems_amd.patches import patch_vllm_all
+
+    seen = []
+    monkeypatch.setattr(importlib.import_module("flaggems_amd.fused.reshape_and_cache_flash"), "reshape_and_cache_flash", lambda *a: seen.append(a))
+    monkeypatch.setattr(importlib.import_module("flaggems_amd.ops.attention"), "flash_attn_varlen_func", lambda **kw: seen.append(kw))
+    one = torch.ones(1)
+    layer = types.SimpleNamespace(_q_scale=one, _k_scale=one, _v_scale=one)
+    meta = types.SimpleNamespace(num_actual_tokens=3, slot_mapping=None, use_cascade=False, query_start_loc=torch.zeros(3), seq_lens=None,
+                                 max_query_len=2, max_seq_len=9, block_table=None, scheduler_metadata=None)
+    impl = types.SimpleNamespace(kv_cache_dtype=name, use_irope=False, scale=1.0, alibi_slopes=None, sliding_window=(-1, -1), logits_soft_cap=0)
+    x = torch.zeros(3, 2, 64)
+    with pytest.raises(NotImplementedError, match=name):
+        patch_vllm_all.custom_gems_flash_attention_impl_forward(impl, layer, x, x, x, torch.zeros(2, 4, 16, 2, 64, dtype=torch.uint8).view(kind), meta, output=x)
+    assert not seen
