@@ -46,7 +46,8 @@ def gather_cache_flash(
     assert key_cache.is_cuda, "the tensors must be on a GPU"
     fmt = _C.cache_format(cache_dtype, kv_cache_dtype)
     if dtype is None:
-        dtype = key.dtype if key is not None else torch.bfloat16 if fmt is not None else cache_dtype
+        given = key if key is not None else value
+        dtype = given.dtype if given is not None else torch.bfloat16 if fmt is not None else cache_dtype
     if fmt is None:
         assert dtype is cache_dtype, "a cache of %s is read back as it is" % cache_dtype
         fmt, k_scale, v_scale = _C.CACHE_SAME, None, None

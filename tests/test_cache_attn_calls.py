@@ -216,3 +216,16 @@ def test_vllm_hook_refuses_caches_it_does_not_know(monkeypatch, name, kind):
     with pytest.raises(NotImplementedError, match=name):
         patch_vllm_all.custom_gems_flash_attention_impl_forward(impl, layer, x, x, x, torch.zeros(2, 4, 16, 2, 64, dtype=torch.uint8).view(kind), meta, output=x)
     assert not seen
+
+
+def test_the_type_of_either_given_output_decides(asked):
+    """An 8-bit cache is read to the type of the outputs that are given, whichever is: bf16 only if none is."""
+    c = torch.zeros(6, 16, 2, 64).to(E4M3)
+    table, cu = torch.zeros(3, 4, dtype=torch.int32), torch.tensor([0, 5, 5, 30], dtype=torch.int32)
+    room = torch.zeros(30, 2, 64)
+    for given in (dict(key=room), dict(value=room), dict(key=room, value=room.clone())):
+        k, v = flag_gems.gather_cache_flash(c, c, table, cu, 30, **given)
+        assert k.dtype == v.dtype == torch.float32
+    with pytest.raises(AssertionError, match="num_rows, heads"):
+        flag_gems.gather_cache_flash(c, c, table, cu, 30, key=room, value=room.half())
+    assert [a[-3] for n, a in asked.calls] == [_C.FG_F32] * 3
