@@ -113,7 +113,13 @@ Plan make_plan(const FgCacheAttnParams& c) {
     return p.window_left >= 0 && window < keys ? window : keys;
   };
   const int few = 32 / G > 1 ? 32 / G : 1;
-  plan.tile = p.D <= 128 && p.max_seqlen_q > few;
+  // The tile kernel's offsets are 32 bits of 16-byte pieces: inside a page, and from one page to the next.
+  const int bytes = c.cache_format == FG_CACHE_SAME ? 2 : 1;
+  auto near = [&](int64_t page, int64_t row) {
+    const int64_t most = (int64_t)1 << 32;
+    return row * bytes / 16 <= (most - 1) / std::max(p.page_size - 1, 1) && (c.num_pages == 1 || page * bytes / 16 < most);
+  };
+  plan.tile = p.D <= 128 && p.max_seqlen_q > few && near(p.k_page_stride, p.k_row_stride) && near(p.v_page_stride, p.v_row_stride);
   plan.stream_q = plan.tile ? few : p.max_seqlen_q;
   // The tile kernel takes the short sequences too where all are as long as the longest, so that there are none, and where no row
   // sees more than 1024 keys: a launch of its own costs more than such a sequence does here.

@@ -229,3 +229,23 @@ def test_the_type_of_either_given_output_decides(asked):
     with pytest.raises(AssertionError, match="num_rows, heads"):
         flag_gems.gather_cache_flash(c, c, table, cu, 30, key=room, value=room.half())
     assert [a[-3] for n, a in asked.calls] == [_C.FG_F32] * 3
+
+
+def test_offsets_beyond_32_bits_stay_with_64_bit_arithmetic(launched):
+    """The chunk kernel counts 16-byte pieces inside a page, and between pages, in 32 bits; pages or strides beyond that (64 GiB)
+    are attended over by the kernel that counts in 64."""
+    def chunk(page, keys, **kw):
+        return sizes(total=600, batch=1, longest=600, keys=keys, page=page, **kw)
+
+    far = [chunk(1 << 26, 1 << 26, hk=16), chunk((1 << 26) + 1, 1 << 26), chunk(1 << 13, 1 << 16, k_row_stride=524353 * 16),
+           chunk(1 << 13, 1 << 16, v_row_stride=1 << 24), chunk(16, 1 << 16, k_page_stride=1 << 36), chunk(16, 1 << 16, v_page_stride=1 << 37),
+           chunk(1 << 12, 1 << 16, fmt=_C.CACHE_SAME, k_row_stride=1 << 24, window=700, sinks=4)]
+    near = [chunk(1 << 26, 1 << 26), chunk(1 << 13, 1 << 16, k_row_stride=524352 * 16), chunk(16, 1 << 16, k_page_stride=(1 << 36) - 16),
+            chunk(1 << 12, 1 << 16, fmt=_C.CACHE_SAME, k_row_stride=1 << 23, window=700, sinks=4),
+            chunk(16, 1 << 16, v_page_stride=1 << 37, num_pages=1)]
+    answers = launched(far + near)
+    kinds = []
+    for i, (rc, text, launches) in enumerate(answers):
+        assert rc == 0, (i, text)
+        kinds.append({"tile" if "attn_tile" in name else "stream" for name, _, _, _ in launches if "attn_merge" not in name})
+    assert kinds == [{"stream"}] * len(far) + [{"tile"}] * len(near)
