@@ -237,10 +237,10 @@ def test_offsets_beyond_32_bits_stay_with_64_bit_arithmetic(launched):
     def chunk(page, keys, **kw):
         return sizes(total=600, batch=1, longest=600, keys=keys, page=page, **kw)
 
-    far = [chunk(1 << 26, 1 << 26, hk=16), chunk((1 << 26) + 1, 1 << 26), chunk(1 << 13, 1 << 16, k_row_stride=524353 * 16),
+    far = [chunk(1 << 26, 1 << 26, hk=16, num_pages=1), chunk((1 << 26) + 1, 1 << 26, num_pages=1), chunk(1 << 13, 1 << 16, k_row_stride=524353 * 16),
            chunk(1 << 13, 1 << 16, v_row_stride=1 << 24), chunk(16, 1 << 16, k_page_stride=1 << 36), chunk(16, 1 << 16, v_page_stride=1 << 37),
            chunk(1 << 12, 1 << 16, fmt=_C.CACHE_SAME, k_row_stride=1 << 24, window=700, sinks=4)]
-    near = [chunk(1 << 26, 1 << 26), chunk(1 << 13, 1 << 16, k_row_stride=524352 * 16), chunk(16, 1 << 16, k_page_stride=(1 << 36) - 16),
+    near = [chunk(1 << 26, 1 << 26, num_pages=1), chunk(1 << 13, 1 << 16, k_row_stride=524352 * 16), chunk(16, 1 << 16, k_page_stride=(1 << 36) - 16),
             chunk(1 << 12, 1 << 16, fmt=_C.CACHE_SAME, k_row_stride=1 << 23, window=700, sinks=4),
             chunk(16, 1 << 16, v_page_stride=1 << 37, num_pages=1)]
     answers = launched(far + near)
