@@ -83,9 +83,11 @@ int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 // Microseconds that a launch of the tile kernel takes with row blocks of 64 * nq rows and `splits` key ranges, from what was
 // measured on MI355X: the steps of a tile on a CU that holds one workgroup or two, start and end of a workgroup, and the merge
 // (its launch, and 2 * (DP + 2) * 4 bytes for each range, token and head at 5 TB/s).  `even`: all sequences as long as the
-// longest; otherwise their blocks are taken to be 0.6 of the longest on average, and a long one to begin among the last.  Chunks
-// of (1024, 765, 284, 14) tokens over (8192, 4816, 3212, 2548) keys, 32/8 heads: 577 us unsplit, 306 in 2 ranges, 312 in 4 (308
-// here), 516 in 12; one chunk of 1000 over 1000: blocks of 64 rows 35 us, of 128 rows 43, in 2 ranges 53 and 55.
+// longest; otherwise their blocks are taken to be 0.6 of the longest on average, and a long one to begin among the last.  Whole
+// calls, chunks of (1024, 765, 284, 14) tokens over (8192, 4816, 3212, 2548) keys, 32/8 heads: blocks of 128 rows 588 us unsplit, 305 in
+// 2 ranges, 303 in 3, 309 in 4 (taken), 328 in 6, 518 in 12; of 64 rows 826, 391 in 2, 400 in 4.  One chunk of 1000 over 1000: blocks
+// of 64 rows 33 us (taken), of 128 rows 42, in 2 ranges 48 and 51.  What the model leaves out is workgroups for rows that are not
+// there, which uneven batches have many of: the merge of the chunks above takes 45 us, its bytes 28.
 double tile_cost(int64_t blocks, double tiles, int nq, int dp, int64_t cus, int splits, bool even, double merge_bytes) {
   const double dim = dp == 64 ? 0.72 : 1.0;
   const double alone = (nq == 1 ? 1.32 : 1.7) * dim, shared = (nq == 1 ? 1.54 : 2.3) * dim;
@@ -122,7 +124,9 @@ Plan make_plan(const FgCacheAttnParams& c) {
   plan.tile = p.D <= 128 && p.max_seqlen_q > few && near(p.k_page_stride, p.k_row_stride) && near(p.v_page_stride, p.v_row_stride);
   plan.stream_q = plan.tile ? few : p.max_seqlen_q;
   // The tile kernel takes the short sequences too where all are as long as the longest, so that there are none, and where no row
-  // sees more than 1024 keys: a launch of its own costs more than such a sequence does here.
+  // sees more than 1024 keys: a launch of its own mostly costs more than such sequences do here.  A chunk of 512 and three tokens over
+  // 512 keys each, 32/8 heads: 38 us here, 48 in two launches; 300 and 15 tokens over up to 900: 53 and 57; 24 sequences of up to 100
+  // over up to 700, 8/2 heads: 25 and 35; 300 and 15 over up to 2000: 77 and 78.  (100 and 63 tokens over 1000: 94 and 79.)
   const bool even = (int64_t)p.total_q >= (int64_t)p.batch * p.max_seqlen_q;
   if (plan.tile && (even || keys_of(fg_cdiv(64, G), kTileKeys) <= 1024)) plan.stream_q = 0;
   const bool pow2 = (p.page_size & (p.page_size - 1)) == 0;
@@ -134,9 +138,10 @@ Plan make_plan(const FgCacheAttnParams& c) {
     const int64_t tiles = fg_cdiv(keys_of(fg_cdiv(16 * plan.nq, G), kTile), kTile);
     const int64_t groups = fg_cdiv((int64_t)plan.stream_q * G, 16 * plan.nq) * p.batch * p.Hk;
     // Two workgroups per CU fill the card.  Below that the keys are cut into ranges for up to four per CU (sequences differ, and
-    // the ranges of a short one end early) of at least 16 tiles, or for one per CU of at least 4: 24 groups of 4096 tiles take
-    // 1400 us unsplit, 138 cut in 16 and 115 in 43; 8 groups of 62 tiles 21 us unsplit, 13 cut in 12; 512 groups of 128 tiles
-    // 105 us unsplit, 108 cut in 3.  Up to 32 tiles the launch that merges costs what the ranges save.
+    // the ranges of a short one end early) of at least 16 tiles, or for one per CU of at least 4.  Whole calls: 24 groups of up to
+    // 4096 tiles take 984 us unsplit, 111 cut in 16 and 107 in 43; 8 groups of 62 tiles 21 us unsplit, 17 cut in 12; 512 groups of
+    // 128 tiles 98 us unsplit, 98 cut in 3.  Up to 32 tiles the launch that merges costs more than the ranges save: 8 groups of 32
+    // take 13.5 us unsplit, 17.3 in 4 or in 8.
     plan.min_tiles = 4;
     int64_t splits = 1;
     if (groups < 2 * cus && tiles > 32) {

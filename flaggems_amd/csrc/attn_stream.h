@@ -32,10 +32,12 @@
 // out = 0, lse = +inf.  A block table entry that names no page of the cache makes the rows that need it NaN.
 //
 // Bound: HBM (2 * D bytes a key for 8 bits, against 4 * D * rows flop; without its arithmetic the loop takes the same time).
-// 32/8 heads of 128, one token: 64 sequences of 4096 keys, e4m3, 98 us = 5.5 TB/s; 256 of them 5.9; three of 131072 keys at most,
-// in ranges, 102 us and 5 for the merge = 5.4 TB/s; 128 of 4096, 16 bits, 6.1 (a large copy on this card: 5.0 to 5.4, loads
-// alone up to 5.5).  One workgroup draws 22 to 28 GB/s on its own, with four waves or eight: a short sequence is bound by that
-// and by the trips to memory one after another (lengths and table, keys, output), 12 us for 513 keys in 8 workgroups.
+// 32/8 heads of 128, one token: 64 sequences of 4096 keys, e4m3, 98 us = 5.5 TB/s; 256 of them 326 = 6.6; three of 131072 keys at most,
+// in ranges, 102 us and 5 for the merge = 5.4 TB/s; 128 of 4096, 16 bits, 329 = 6.5 (a large copy on this card: 4.8 to 5.4).  Head
+// dim 256, 64 of 4096: e4m3 179 us = 6.0 TB/s, 16 bits (loaded where they are used) 459 = 4.7.  Chunks of head dims above 128 come
+// here too and read the keys again for every 16 rows: 1024 tokens over 8192, dim 256, 744 us = 0.35 PFLOP/s, 16 bits 2.65 ms = 0.10.
+// One workgroup draws 22 to 28 GB/s on its own, with four waves or eight: a short sequence is bound by that and by the trips
+// to memory one after another (lengths and table, keys, output), 12 us for 513 keys in 8 workgroups.
 // What the loads are made of decides: 32 bytes a lane at a stretch, in place of whole 128-byte lines, cost a fifth.
 #pragma once
 

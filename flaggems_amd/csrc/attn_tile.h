@@ -17,11 +17,11 @@
 //
 // Bound: matrix pipe and vector ALU together (32 MFMA of 16 clocks against 16 exponentials of 16 clocks and some 40 plain
 // instructions of 4 per wave and 32 keys); two workgroups per CU, so that one wave's softmax runs under another's products.
-// 32/8 heads of 128, e4m3: 8 x 2048 tokens over 8192 keys 2.10 ms = 0.92 PFLOP/s, 8192 over themselves 0.88; four chunks of up to
-// 1024 over up to 8192, in two ranges, 300 us and 50 for the merge = 0.64 (with the merge; uneven, one round of workgroups).
-// 16 bits, 8192 tokens under a window of 1024 keys and 4 sinks: 245 us = 0.53 PFLOP/s of visible keys (19 tiles a block, of which
-// two or three are partly masked).  Counters there: matrix pipe busy 22 % of the time, no LDS conflicts.  With 8 bits a
-// quarter of the LDS cycles are conflicts of the staging writes; places without them (the halves of a row apart) gain 1 % there
+// 32/8 heads of 128, e4m3: 8 x 2048 tokens over 8192 keys 2.10 ms = 0.92 PFLOP/s, 8192 over themselves 625 us = 0.88; four chunks of
+// up to 1024 over up to 8192, in four ranges, 262 us = 0.76 and 45 for the merge (0.64 with everything; uneven, one round of workgroups).
+// 16 bits, 8192 tokens under a window of 1024 keys and 4 sinks: 246 us = 0.53 PFLOP/s of visible keys (19 tiles a block, of which
+// two or three are partly masked).  (After a third of a second of such calls; the first ones after a pause take a sixth longer.)
+// Counters there: matrix pipe busy 22 % of the time, no LDS conflicts.  With 8 bits a quarter of the LDS cycles are conflicts of the staging writes; places without them (the halves of a row apart) gain 1 % there
 // and cost the 16-bit reads 7 %.
 #pragma once
 

@@ -266,7 +266,7 @@ int read_launch(const ReadArgs& a, hipStream_t st) {
   return fg_check_launch("gather_cache_flash");
 }
 
-// 85 thousand rows of [8, 128], K and V, e4m3 to bf16: 91 us = 5.75 TB/s (two thirds of it stores, which alone reach 6.8).
+// 85 thousand rows of [8, 128], K and V, e4m3 to bf16: 90 us = 5.8 TB/s (two thirds of it stores, which alone reach 6.8).
 // Pieces of 16 output bytes, one stretch over the wave (pieces of 32 bytes were a fifth slower), where everything is aligned for
 // them, else single elements.
 template <typename U, int FMT>

@@ -151,7 +151,7 @@ def cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, page_table, alibi_slop
                    softmax_scale, is_causal, window_size_left, window_size_right, softcap, num_sink_tokens, k_descale,
                    v_descale, return_lse=True):
     """Attention over an 8-bit paged cache, or under a window with sink tokens: validation + launch.  Returns (out, lse);
-    lse is None where it is not asked for."""
+    lse is None where it is not asked for.  Takes scratch memory for the call, 1.05 GiB at most, and runs without if there is none."""
     assert q.is_cuda and k.is_cuda and v.is_cuda
     dtype, cache_dtype, index = q.dtype, k.dtype, q.get_device()
     assert dtype is torch.bfloat16 or dtype is torch.float16, "FlashAttention only support fp16 and bf16 data type"
@@ -275,8 +275,9 @@ def flash_attn_varlen_func(
     (batch, nheads_k), None for 1.  q stays in 16 bits (q_descale must be None).
     num_sink_tokens: the first keys of a sequence stay visible in front of a left window (key j is visible if it lies in the
     window or j < num_sink_tokens, and the causal or right bound admits it); pages outside both are not read and may be gone.
-    Neither goes together with alibi_slopes.  A block table entry that is needed and names no page of the cache gives NaN;
-    so does an infinite or NaN value, for the queries that see its key and for others that share their block of rows.
+    Neither goes together with alibi_slopes.  A block table entry that is needed and names no page of the cache gives NaN.  An
+    infinite or NaN value in V gives NaN or infinities to the queries that see its key and to others that share their block
+    of rows; in K, NaN to the queries whose score it makes NaN or +infinity.
     """
     logger.debug("GEMS FLASH_ATTN_VARLEN_FUNC")
     assert cu_seqlens_k is not None or seqused_k is not None, "cu_seqlens_k or seqused_k must be provided"

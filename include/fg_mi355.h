@@ -325,8 +325,8 @@ typedef struct FgCacheAttnParams {
  * The reference accepts the descale arguments and ignores them (src/flag_gems/ops/attention.py:1118-1287). */
 int fg_cache_attn_fwd(const FgCacheAttnParams* p /*host*/, void* stream);
 
-/* Scratch the forward would like: partial results of split key ranges.  Without it (NULL or too small) it runs unsplit.
- * Uninitialised memory is fine; one stream at a time. */
+/* Scratch the forward would like: partial results of split key ranges, 1.05 GiB at most.  Without it (NULL or too small) it runs
+ * unsplit.  Uninitialised memory is fine; one stream at a time.  0 also for parameters that the forward refuses. */
 size_t fg_cache_attn_workspace_bytes(const FgCacheAttnParams* p /*host*/, int device);
 
 /* ------------------------------------------------------------------------------------------------------------
