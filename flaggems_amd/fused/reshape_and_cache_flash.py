@@ -24,10 +24,10 @@ def reshape_and_cache_flash(
     the inner [heads, head_size] block of a token must be dense.
 
     An 8-bit cache (torch.float8_e4m3fn or torch.float8_e5m2, with kv_cache_dtype "auto" or the name of that format, or
-    torch.uint8 with "fp8", "fp8_e4m3", which are one format, or "fp8_e5m2") takes clamp(row / scale) rounded to the nearest
-    value of the format, ties to even; infinities become the largest value, NaN stays NaN.  k_scale / v_scale: float32
-    tensors of one number or one for each head, None for 1.  Rows are fp16, bf16 or fp32.  A slot outside the cache is skipped
-    like a negative one; slots must differ."""
+    torch.uint8 with "fp8", "fp8_e4m3", which are one format, or "fp8_e5m2") takes clamp(row / scale), a float32 quotient,
+    rounded to the nearest value of the format, ties to even; infinities become the largest value, NaN stays NaN.  k_scale /
+    v_scale: float32 tensors of one number or one for each head, None for 1.  Rows are fp16, bf16 or fp32.  A slot outside
+    the cache is skipped like a negative one; slots must differ."""
     logger.debug("GEMS RESHAPE_AND_CACHE_FLASH")
     if key_cache.dtype in _C.CACHE_8BIT and key.dtype is not key_cache.dtype:
         return _quantize_and_cache(key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale)

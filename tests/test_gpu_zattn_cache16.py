@@ -54,3 +54,23 @@ def test_chunks_in_more_than_eight_ranges(gpu, monkeypatch, dtype, fmt, window, 
     assert list(kept.values())[0] > 8 * tokens * 8 * (dim + 2) * 4
     again = run_and_check(gpu, lens, 8, 2, dim, 16, dtype, fmt, window=window, sinks=sinks)
     assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("lens", [[(1, 700), (1, 33)], [(90, 300), (2, 40)]], ids=["tokens", "chunks"])
+@pytest.mark.parametrize("softmax_scale,k_scale,v_scale", [(-0.1, 0.05, 0.05), (0.1, -0.05, -0.04), (-0.1, -0.05, 0.04), (0.0, 0.05, 0.05), (0.1, 0.0, 0.04),
+                                                           (0.1, 0.05, 0.0), (1e-3, 5.0, 1e-30), (1e20, 5e-22, 1e30)])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_signs_and_sizes_of_scales(gpu, lens, softmax_scale, k_scale, v_scale, softcap):
+    """The kernels move the sign of the score's factor into the query, and a factor of 0 makes every visible key weigh the same."""
+    import flag_gems
+    from oracle import torch_ref as O
+    from test_gpu_zattn_cache import assert_close, make
+
+    q, kc, vc, cu, used, table, _, _ = make(gpu, lens, 8, 2, 64, 16, torch.bfloat16, "e4m3", scales="none")
+    ks, vs = torch.tensor([k_scale], device=gpu), torch.tensor([v_scale], device=gpu)
+    out, lse = flag_gems.flash_attn_varlen_func(q, kc, vc, max(n for n, _ in lens), cu, max(k for _, k in lens), seqused_k=used, causal=True, block_table=table,
+                                                softmax_scale=softmax_scale, softcap=softcap, k_descale=ks, v_descale=vs, return_softmax_lse=True)
+    ref = O.cache_attention(q, kc, vc, cu, used, table, softmax_scale, softcap=softcap, k_scale=ks, v_scale=vs)
+    # (sum |q| |k| times the factor's size: the oracle's bound takes the factor with its sign)
+    size = O.cache_attention(q.abs(), kc.view(torch.uint8).bitwise_and(127).view(kc.dtype), vc, cu, used, table, abs(softmax_scale), k_scale=ks.abs())
+    assert_close(out, lse, dict(ref, reach=size["reach"].abs()), torch.bfloat16, 64)
