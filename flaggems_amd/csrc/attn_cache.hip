@@ -119,7 +119,7 @@ Plan make_plan(const FgCacheAttnParams& c) {
   const int bytes = c.cache_format == FG_CACHE_SAME ? 2 : 1;
   auto near = [&](int64_t page, int64_t row) {
     const int64_t most = (int64_t)1 << 32;
-    return row * bytes / 16 <= (most - 1) / std::max(p.page_size - 1, 1) && (c.num_pages == 1 || page * bytes / 16 < most);
+    return (p.page_size == 1 || row * bytes / 16 <= (most - 1) / (p.page_size - 1)) && (c.num_pages == 1 || page * bytes / 16 < most);
   };
   plan.tile = p.D <= 128 && p.max_seqlen_q > few && near(p.k_page_stride, p.k_row_stride) && near(p.v_page_stride, p.v_row_stride);
   plan.stream_q = plan.tile ? few : p.max_seqlen_q;

@@ -141,7 +141,7 @@ def mha_varlan_fwd(
     return out, q, k, v, lse, philox_args, unused, probs
 
 
-# Scratch sizes by everything they depend on: sizes, masks and the device (one library call less for a shape seen before).
+# Scratch sizes by everything they depend on: sizes, masks, the caches' layout and the device (one library call less for a shape seen before).
 # Kept of calls that ran only: the library also answers 0 for parameters that it refuses, for reasons that are not in the key.
 _cache_attn_scratch = {}
 _INT32_MAX = 2 ** 31 - 1
@@ -208,7 +208,7 @@ def cache_attn_fwd(q, k, v, out, cu_seqlens_q, seqused_k, page_table, alibi_slop
                 *sizes, softmax_scale, softcap, _C.dtype_id(dtype), ws, ws_bytes, fmt, num_sink_tokens, num_pages, table_width,
                 k_scale[0], v_scale[0], k_scale[1], k_scale[2], v_scale[1], v_scale[2])
 
-        key = (sizes, total_q, num_sink_tokens, fmt, index)
+        key = (sizes, total_q, num_sink_tokens, fmt, index, num_pages, k_page, k_row, v_page, v_row)
         ws_bytes = _cache_attn_scratch.get(key)
         if ws_bytes is None:
             ws_bytes = _C.lib().fg_cache_attn_workspace_bytes(packed(0, 0), index)

@@ -242,7 +242,7 @@ def test_offsets_beyond_32_bits_stay_with_64_bit_arithmetic(launched):
            chunk(1 << 12, 1 << 16, fmt=_C.CACHE_SAME, k_row_stride=1 << 24, window=700, sinks=4)]
     near = [chunk(1 << 26, 1 << 26, num_pages=1), chunk(1 << 13, 1 << 16, k_row_stride=524352 * 16), chunk(16, 1 << 16, k_page_stride=(1 << 36) - 16),
             chunk(1 << 12, 1 << 16, fmt=_C.CACHE_SAME, k_row_stride=1 << 23, window=700, sinks=4),
-            chunk(16, 1 << 16, v_page_stride=1 << 37, num_pages=1)]
+            chunk(16, 1 << 16, v_page_stride=1 << 37, num_pages=1), chunk(1, 1 << 16, k_row_stride=1 << 40)]
     answers = launched(far + near)
     kinds = []
     for i, (rc, text, launches) in enumerate(answers):
